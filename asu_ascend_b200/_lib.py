@@ -8,7 +8,7 @@ libcudart.so.12 dependency binds to the CUDA runtime torch already loaded.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
@@ -32,10 +32,13 @@ STATUS_BITS = {
     0x40: "BAD_TOKEN_STATE",
     0x80: "NO_VICTIM",
     0x100: "TIMEOUT",
+    0x200: "BAD_WEIGHT",
 }
 ST_BAD_QUERY, ST_FREE_EXHAUSTED, ST_RING_EXHAUSTED, ST_BAD_STATE = 0x01, 0x02, 0x04, 0x08
 ST_SHORTAGE, ST_BAD_SOURCE, ST_BAD_TOKEN_STATE, ST_NO_VICTIM = 0x10, 0x20, 0x40, 0x80
-ST_TIMEOUT = 0x100
+ST_TIMEOUT, ST_BAD_WEIGHT = 0x100, 0x200
+
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 
 LRU_STAT_COLS = 5
 
@@ -85,8 +88,16 @@ _SIGS = {
     "asu_resolver_mark_token": [_P, c_int64, _P, c_int64, c_int64],
     "asu_kv_resolver_lru": [_P, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P,
                             _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P, _P],
+    "asu_kv4_pack": [_P, _P, c_int32, c_int64, c_int64, _P, _P, c_int64, c_uint64, _P],
+    "asu_kv4_unpack": [_P, _P, c_int64, c_uint64, _P, c_int64, _P, c_int64, _P],
+    "asu_kv4_attention_workspace_bytes": [c_int64, c_int64, c_int64, c_int32],
+    "asu_kv4_attention": [_P, _P, c_int64, c_int64, _P, c_int64, c_uint64, c_uint64, _P, c_int64, c_int64, c_int64,
+                          c_int64, c_float, _P, _P, _P, _P, c_int64, _P],
+    "asu_weight_step": [_P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_uint32, c_float, _P, _P, _P, _P, _P, _P, c_uint32,
+                        _P, _P, _P, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32],
 }
-_RESTYPE = {"asu_status_string": c_char_p, "asu_kv_resolver_workspace_bytes": c_int64}
+_RESTYPE = {"asu_status_string": c_char_p, "asu_kv_resolver_workspace_bytes": c_int64,
+            "asu_kv4_attention_workspace_bytes": c_int64}
 
 
 class AsuError(RuntimeError):

@@ -28,7 +28,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <optional>
 #include <sstream>
 #include <tuple>
@@ -41,13 +43,14 @@ namespace {
 std::atomic<bool> g_status_checks{false};
 
 const char* const kStatusNames[] = {"BAD_QUERY",  "FREE_EXHAUSTED", "RING_EXHAUSTED",  "BAD_STATE", "SHORTAGE",
-                                    "BAD_SOURCE", "BAD_TOKEN_STATE", "NO_VICTIM", "TIMEOUT"};
+                                    "BAD_SOURCE", "BAD_TOKEN_STATE", "NO_VICTIM", "TIMEOUT",
+                                    "BAD_WEIGHT"};
 
 std::string status_list(int bits) {
     std::ostringstream os;
     os << "[";
     bool first = true;
-    for (int i = 0; i < 9; ++i) {
+    for (int i = 0; i < 10; ++i) {
         if (bits & (1 << i)) {
             os << (first ? "" : ", ") << "'" << kStatusNames[i] << "'";
             first = false;
@@ -449,6 +452,174 @@ constexpr const char* kSimtSchema =
     "Tensor query_token_ids, int req_num) -> (Tensor, Tensor)";
 
 // ---------------------------------------------------------------------------------------------
+// 4-bit MLA cache (this library's own operators: registered under `asu` only)
+
+// Rows of a 4-bit pool: [rows, 416] bytes, or [tokens, rows, 416] with one pool per token.
+void check_kv4_pool(const at::Tensor& pool, const c10::Device& dev, bool per_token) {
+    TORCH_CHECK(pool.scalar_type() == at::kByte, "pool must be uint8");
+    TORCH_CHECK(pool.device() == dev, "pool must be on ", dev, ", got ", pool.device());
+    TORCH_CHECK(pool.dim() == 2 || (per_token && pool.dim() == 3), "pool must be [rows, 416]",
+                per_token ? " or [tokens, rows, 416]" : "", ", got ", pool.sizes());
+    TORCH_CHECK(pool.size(-1) == ASU_KV4_ROW_BYTES && pool.stride(-1) == 1,
+                "pool rows must be 416 contiguous bytes, got ", pool.size(-1), " with stride ", pool.stride(-1));
+    TORCH_CHECK(pool.size(-2) > 0, "pool has no rows");
+    TORCH_CHECK(pool.stride(-2) >= ASU_KV4_ROW_BYTES || pool.size(-2) == 1, "pool rows must not overlap");
+    TORCH_CHECK(pool.stride(-2) % 16 == 0 && reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0 &&
+                    (pool.dim() == 2 || pool.stride(0) % 16 == 0),
+                "pool rows must start at multiples of 16 bytes");
+}
+
+// Bytes between pool rows; a pool of one row may carry any stride.
+uint64_t kv4_pitch(const at::Tensor& pool) {
+    return static_cast<uint64_t>(std::max<int64_t>(pool.stride(-2), ASU_KV4_ROW_BYTES));
+}
+
+void check_kv4_slots(const at::Tensor& slots, const c10::Device& dev) {
+    TORCH_CHECK(slots.scalar_type() == at::kInt, "slots must be int32");
+    TORCH_CHECK(slots.device() == dev, "slots must be on ", dev, ", got ", slots.device());
+}
+
+void no_grad_needed(const at::Tensor& t, const char* name) {
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+                " requires a gradient, and the 4-bit cache's operators have none: call them under torch.no_grad()");
+}
+
+void kv4_pack_checks(const at::Tensor& src, const at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    const c10::Device dev = src.device();
+    TORCH_CHECK(src.scalar_type() == at::kBFloat16 || src.scalar_type() == at::kHalf, "src must be bfloat16 or float16");
+    TORCH_CHECK(src.dim() == 2 && src.size(1) == ASU_KV4_LATENT + ASU_KV4_ROPE, "src must be [n, 576], got ",
+                src.sizes());
+    TORCH_CHECK(src.stride(1) == 1 || src.numel() == 0, "src rows must be contiguous");
+    no_grad_needed(src, "src");
+    check_kv4_pool(pool, dev, false);
+    if (slots.has_value()) {
+        check_kv4_slots(*slots, dev);
+        TORCH_CHECK(slots->dim() == 1 && slots->is_contiguous() && slots->size(0) == src.size(0),
+                    "slots must be a contiguous [n] tensor, one per row of src");
+    } else {
+        TORCH_CHECK(src.size(0) <= pool.size(0), "src has more rows than the pool");
+    }
+}
+
+void kv4_pack_cuda(const at::Tensor& src, at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    kv4_pack_checks(src, pool, slots);
+    const int64_t n = src.size(0);
+    if (n == 0) return;
+    const c10::cuda::CUDAGuard guard(src.device());
+    const at::Tensor status = new_status(1, pool);
+    launch_ok(asu_kv4_pack(c10::cuda::getCurrentCUDAStream(src.device().index()).stream(), src.data_ptr(),
+                           src.scalar_type() == at::kHalf ? ASU_DTYPE_FP16 : ASU_DTYPE_BF16, src.stride(0), n,
+                           slots.has_value() ? slots->data_ptr<int32_t>() : nullptr, pool.data_ptr(), pool.size(0),
+                           kv4_pitch(pool), status_ptr(status)),
+              "kv4_pack_rows");
+    raise_on_status(status, "kv4_pack_rows");
+}
+
+void kv4_unpack_checks(const at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    check_kv4_pool(pool, pool.device(), false);
+    if (slots.has_value()) {
+        check_kv4_slots(*slots, pool.device());
+        TORCH_CHECK(slots->dim() == 1 && slots->is_contiguous(), "slots must be a contiguous [n] tensor");
+    }
+}
+
+at::Tensor kv4_unpack_cuda(const at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    kv4_unpack_checks(pool, slots);
+    const c10::cuda::CUDAGuard guard(pool.device());
+    const int64_t n = slots.has_value() ? slots->size(0) : pool.size(0);
+    at::Tensor rows = at::empty({n, ASU_KV4_LATENT + ASU_KV4_ROPE}, pool.options().dtype(at::kBFloat16));
+    if (n == 0) return rows;
+    const at::Tensor status = new_status(1, pool);
+    launch_ok(asu_kv4_unpack(c10::cuda::getCurrentCUDAStream(pool.device().index()).stream(), pool.data_ptr(),
+                             pool.size(0), kv4_pitch(pool), slots.has_value() ? slots->data_ptr<int32_t>() : nullptr,
+                             n, rows.data_ptr(), rows.stride(0), status_ptr(status)),
+              "kv4_unpack_rows");
+    raise_on_status(status, "kv4_unpack_rows");
+    return rows;
+}
+
+void kv4_decode_checks(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& slots, double scale) {
+    const c10::Device dev = q.device();
+    TORCH_CHECK(q.scalar_type() == at::kBFloat16, "q must be bfloat16");
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == ASU_KV4_LATENT + ASU_KV4_ROPE, "q must be [tokens, heads, 576], got ",
+                q.sizes());
+    TORCH_CHECK(q.stride(2) == 1 || q.numel() == 0, "q's last dimension must be contiguous");
+    TORCH_CHECK(q.size(1) >= 1 && q.size(1) <= ASU_KV4_MAX_HEADS, "heads must be in [1, 128], got ", q.size(1));
+    TORCH_CHECK(q.size(0) <= ASU_KV4_MAX_TOKENS, "at most 65535 tokens a call, got ", q.size(0));
+    no_grad_needed(q, "q");
+    check_kv4_pool(pool, dev, true);
+    TORCH_CHECK(pool.dim() == 2 || pool.size(0) == q.size(0), "pool has ", pool.size(0), " pools for ", q.size(0),
+                " tokens");
+    TORCH_CHECK(pool.size(-2) <= 0x7fffffff, "pool has too many rows for int32 slots");
+    check_kv4_slots(slots, dev);
+    TORCH_CHECK(slots.dim() == 2 && slots.size(0) == q.size(0), "slots must be [tokens, topk], got ", slots.sizes());
+    TORCH_CHECK(slots.stride(1) == 1 || slots.size(1) <= 1 || slots.size(0) == 0, "slots rows must be contiguous");
+    TORCH_CHECK(slots.size(1) <= ASU_KV4_MAX_TOPK, "at most 16384 entries a token, got ", slots.size(1));
+    TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0.0f,
+                      "scale must be positive and finite");
+}
+
+// (out, lse, weights); weights is empty unless asked for.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv4_decode_cuda(const at::Tensor& q, const at::Tensor& pool,
+                                                               const at::Tensor& slots, double scale, bool weights) {
+    kv4_decode_checks(q, pool, slots, scale);
+    const c10::cuda::CUDAGuard guard(q.device());
+    const int64_t T = q.size(0), H = q.size(1), K = slots.size(1);
+    at::Tensor out = at::empty({T, H, ASU_KV4_LATENT}, q.options());
+    at::Tensor lse = at::empty({T, H}, q.options().dtype(at::kFloat));
+    at::Tensor w = at::empty({weights ? T : 0, K}, q.options());
+    if (T == 0) return {out, lse, w};
+    // of this call alone, from the caching allocator: a captured graph's call gets its own from the graph's pool
+    const int64_t size = asu_kv4_attention_workspace_bytes(T, H, K, weights);
+    at::Tensor ws = at::empty({size}, pool.options());
+    const at::Tensor status = new_status(1, slots);
+    launch_ok(asu_kv4_attention(c10::cuda::getCurrentCUDAStream(q.device().index()).stream(), q.data_ptr(),
+                                q.stride(0), q.stride(1), pool.data_ptr(), pool.size(-2), kv4_pitch(pool),
+                                pool.dim() == 3 ? static_cast<uint64_t>(pool.stride(0)) : 0,
+                                slots.data_ptr<int32_t>(), slots.stride(0), T, H, K, static_cast<float>(scale),
+                                out.data_ptr(), lse.data_ptr<float>(), weights && K ? w.data_ptr() : nullptr,
+                                size ? ws.data_ptr() : nullptr, size, status_ptr(status)),
+              "kv4_sparse_decode");
+    raise_on_status(status, "kv4_sparse_decode");
+    return {out, lse, w};
+}
+
+void kv4_pack_cpu(const at::Tensor& src, at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    kv4_pack_checks(src, pool, slots);
+    TORCH_CHECK(false, "kv4_pack_rows needs CUDA tensors (asu_ascend_b200 has no CPU implementation)");
+}
+
+at::Tensor kv4_unpack_cpu(const at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    kv4_unpack_checks(pool, slots);
+    TORCH_CHECK(false, "kv4_unpack_rows needs CUDA tensors (asu_ascend_b200 has no CPU implementation)");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv4_decode_cpu(const at::Tensor& q, const at::Tensor& pool,
+                                                              const at::Tensor& slots, double scale, bool) {
+    kv4_decode_checks(q, pool, slots, scale);
+    TORCH_CHECK(false, "kv4_sparse_decode needs CUDA tensors (asu_ascend_b200 has no CPU implementation)");
+}
+
+void kv4_pack_meta(const at::Tensor&, at::Tensor&, const std::optional<at::Tensor>&) {}
+
+at::Tensor kv4_unpack_meta(const at::Tensor& pool, const std::optional<at::Tensor>& slots) {
+    return at::empty({slots.has_value() ? slots->size(0) : pool.size(0), ASU_KV4_LATENT + ASU_KV4_ROPE},
+                     pool.options().dtype(at::kBFloat16));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv4_decode_meta(const at::Tensor& q, const at::Tensor&,
+                                                               const at::Tensor& slots, double, bool weights) {
+    return {at::empty({q.size(0), q.size(1), ASU_KV4_LATENT}, q.options()),
+            at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)),
+            at::empty({weights ? q.size(0) : 0, slots.size(1)}, q.options())};
+}
+
+constexpr const char* kKv4PackSchema = "kv4_pack_rows(Tensor src, Tensor(a!) pool, Tensor? slots=None) -> ()";
+constexpr const char* kKv4UnpackSchema = "kv4_unpack_rows(Tensor pool, Tensor? slots=None) -> Tensor";
+constexpr const char* kKv4DecodeSchema =
+    "kv4_sparse_decode(Tensor q, Tensor pool, Tensor slots, float scale, bool weights=False) -> (Tensor, Tensor, Tensor)";
+
+// ---------------------------------------------------------------------------------------------
 
 constexpr const char* kSchema =
     "npu_asu_resolve_kv_slots_single_req(Tensor original_topk_indices, int actual_seq_len, int managed_prefix_len, "
@@ -491,6 +662,27 @@ TORCH_LIBRARY_FRAGMENT(asu, m) { m.def(kLruSchema); }
 TORCH_LIBRARY_IMPL(asu, CUDA, m) { m.impl("npu_asu_resolve_kv_slots_lru", &resolve_lru_cuda); }
 TORCH_LIBRARY_IMPL(asu, CPU, m) { m.impl("npu_asu_resolve_kv_slots_lru", &resolve_lru_cpu); }
 TORCH_LIBRARY_IMPL(asu, Meta, m) { m.impl("npu_asu_resolve_kv_slots_lru", &resolve_lru_meta); }
+
+TORCH_LIBRARY_FRAGMENT(asu, m) {
+    m.def(kKv4PackSchema);
+    m.def(kKv4UnpackSchema);
+    m.def(kKv4DecodeSchema);
+}
+TORCH_LIBRARY_IMPL(asu, CUDA, m) {
+    m.impl("kv4_pack_rows", &kv4_pack_cuda);
+    m.impl("kv4_unpack_rows", &kv4_unpack_cuda);
+    m.impl("kv4_sparse_decode", &kv4_decode_cuda);
+}
+TORCH_LIBRARY_IMPL(asu, CPU, m) {
+    m.impl("kv4_pack_rows", &kv4_pack_cpu);
+    m.impl("kv4_unpack_rows", &kv4_unpack_cpu);
+    m.impl("kv4_sparse_decode", &kv4_decode_cpu);
+}
+TORCH_LIBRARY_IMPL(asu, Meta, m) {
+    m.impl("kv4_pack_rows", &kv4_pack_meta);
+    m.impl("kv4_unpack_rows", &kv4_unpack_meta);
+    m.impl("kv4_sparse_decode", &kv4_decode_meta);
+}
 
 // Status checks of the op (synchronise after each call and raise on a device status); the Python
 // side's ops.set_status_checks() forwards here.

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import torch
 
+from . import kv4
 from . import manager as _manager
 from ._lib import ST_BAD_QUERY, check, lib, raise_on_status
 from .ops import status_checks_enabled
@@ -114,16 +115,19 @@ def resolve_topk(ctx: _manager.ASULayerKVCacheContext, topk_indices: torch.Tenso
 def sparse_mla_decode(q: torch.Tensor, ctx: _manager.ASULayerKVCacheContext, topk_indices: torch.Tensor,
                       block_table: torch.Tensor, kv_cache: torch.Tensor, softmax_scale: float,
                       head_padding: int = 128) -> torch.Tensor:
-    """One request's sparse-MLA decode over the managed cache: resolve, then FlashMLA-sparse.
+    """One request's sparse-MLA decode over the managed cache: resolve, then FlashMLA-sparse, or the
+    4-bit attention (``kv4.sparse_decode``) where the cache's rows are 4-bit rows (uint8, 416 bytes).
 
-    q: ``[num_tokens, num_heads, 576]`` bf16; returns ``[num_tokens, num_heads, 512]``.  Heads are
-    padded to a multiple of ``head_padding`` (128 on Blackwell) as vLLM's bf16 path does
-    (flashmla_sparse.py:961-990).
+    q: ``[num_tokens, num_heads, 576]`` bf16; returns ``[num_tokens, num_heads, 512]``.  For
+    FlashMLA-sparse heads are padded to a multiple of ``head_padding`` (128 on Blackwell) as vLLM's
+    bf16 path does (flashmla_sparse.py:961-990).
     """
-    from vllm.third_party.flashmla.flash_mla_interface import flash_mla_sparse_fwd
-
     slots = resolve_topk(ctx, topk_indices, block_table, kv_cache)
     t, h, d = q.shape
+    if kv_cache.dtype == torch.uint8 and kv_cache.shape[2] == kv4.ROW_BYTES:
+        return kv4.sparse_decode(q, ctx.managed_kv_cache_0, slots.view(t, -1), softmax_scale).out
+    from vllm.third_party.flashmla.flash_mla_interface import flash_mla_sparse_fwd
+
     if h % head_padding:
         hp = (h + head_padding - 1) // head_padding * head_padding
         qp = q.new_zeros((t, hp, d))

@@ -47,6 +47,7 @@ extern "C" {
 #define ASU_ST_TIMEOUT 0x100        /* swap-in: a bulk copy did not complete within its wait limit (rows skipped);
                                        a late copy may still land in shared memory, so the stream's later
                                        results are not to be trusted: handle it like a context error */
+#define ASU_ST_BAD_WEIGHT 0x200     /* weight step: a negative, infinite or NaN attention weight was not added */
 
 /* ---- reference constants (ops/asu_hbm_index_lookup_aiv.cpp:7-12) ------- */
 #define ASU_HBM_INDEX_SIZE (128u * 1024u)
@@ -68,6 +69,20 @@ extern "C" {
 #define ASU_TOKEN_ASU_ONLY 0
 #define ASU_TOKEN_HBM_RESIDENT 1
 #define ASU_TOKEN_TAIL_HBM 2
+
+/* Element types of the entry points that take more than one. */
+#define ASU_DTYPE_BF16 0
+#define ASU_DTYPE_FP16 1
+#define ASU_DTYPE_FP32 2
+
+/* The 4-bit MLA row (asu_kv4_*): 512 latent values in 4 bits, 32 scale bytes, 64 bf16 rope values. */
+#define ASU_KV4_LATENT 512
+#define ASU_KV4_ROPE 64
+#define ASU_KV4_GROUP 16
+#define ASU_KV4_ROW_BYTES 416
+#define ASU_KV4_MAX_HEADS 128
+#define ASU_KV4_MAX_TOKENS 65535
+#define ASU_KV4_MAX_TOPK 16384
 
 int asu_version(void);
 const char* asu_status_string(int code);
@@ -380,6 +395,82 @@ int asu_kv_resolver_noalloc(void* stream, const int32_t* topk, int64_t topk_nume
                             const void* kv1_src, void* kv0_dst, void* kv1_dst, int64_t kv0_row_bytes,
                             int64_t kv1_row_bytes, int64_t src_rows, int64_t slot_count, int64_t max_seq_len,
                             int64_t actual_seq_len, int64_t block_size, int32_t* resolved, int32_t* status);
+
+/* ======================================================================
+ * 4-bit MLA cache: rows of 416 bytes, and sparse attention over them
+ * ====================================================================
+ * No reference counterpart: the reference's managed caches hold bf16 rows.  A row stands for 512
+ * latent and 64 position-encoded ("rope") values:
+ *   [0, 256)    nibbles n in 1..15, value (n - 8) * s; eight values share a 32-bit word, value 2j
+ *               as nibble j and value 2j + 1 as nibble j + 4
+ *   [256, 288)  scale bytes b, one per 16 values: s = (1 + (b & 7) / 8) * 2^((b >> 3) - 18)
+ *   [288, 416)  64 bf16 rope values
+ * Rows are raw bytes to asu_swapin_gather, asu_host_pool_writeback and the resolvers, which move
+ * them like any other 416-byte row.  Pools: base and pitch multiples of 16, pitch >= 416. */
+
+/* pool[slots ? slots[i] : i] = row of src[i] (576 values of src_dtype ASU_DTYPE_BF16 / _FP16, rows
+ * src_pitch elements apart) for i < n.  Per group of 16 with a = max |x|: s = a / 7 rounded to three
+ * bits behind the point (ties to even, clamped to the byte's range), n = clamp(rint(x / s), -7, 7)
+ * + 8.  slots[i] = -1 skips row i; any other slot outside [0, pool_rows) sets ASU_ST_BAD_QUERY in
+ * status[0] (nullable) and is skipped.  A latent NaN is stored as 0 and an infinity as the largest
+ * value, with ASU_ST_BAD_SOURCE.  The slots of one call must be distinct. */
+int asu_kv4_pack(void* stream, const void* src, int32_t src_dtype, int64_t src_pitch, int64_t n,
+                 const int32_t* slots, void* pool, int64_t pool_rows, uint64_t pool_pitch, int32_t* status);
+
+/* dst[i] (576 bf16, rows dst_pitch elements apart: a multiple of 8) = the values of pool row
+ * slots ? slots[i] : i, exactly; zeros for slot -1, and for any other slot outside the pool, which
+ * sets ASU_ST_BAD_QUERY. */
+int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows, uint64_t pool_pitch, const int32_t* slots,
+                   int64_t n, void* dst, int64_t dst_pitch, int32_t* status);
+
+/* Sparse MLA attention of `tokens` decode tokens with `heads` heads over 4-bit rows.  Token t reads the
+ * rows slots[t, 0..topk) of the pool at pool + t * pool_token_stride bytes (0: one pool for all),
+ * with -1 for an entry that is not there:
+ *   s_hj = scale * q_th . k_j,  p = softmax over the entries,  out_th = sum_j p_hj v_j,
+ *   lse_th = log sum_j exp s_hj,  weights_tj = sum_h p_hj
+ * with k_j all 576 values and v_j the first 512.  q: bf16, strides in elements; out [tokens, heads,
+ * 512] bf16; lse [tokens, heads] fp32; weights [tokens, topk] bf16 (nullable).  A token without any
+ * entry gets out 0, lse -inf and weights 0.  Any other slot outside [0, pool_rows) counts as not
+ * there and sets ASU_ST_BAD_QUERY in status[0] (nullable).  `workspace`: device memory of
+ * asu_kv4_attention_workspace_bytes(...) bytes on the current device, 16-byte aligned, used by this
+ * call alone until it is done (-1: sizes out of range).  Results do not depend on scheduling.
+ * Limits: heads <= 128, tokens <= 65535, topk <= 16384. */
+int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights);
+int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* pool,
+                      int64_t pool_rows, uint64_t pool_pitch, uint64_t pool_token_stride, const int32_t* slots,
+                      int64_t slots_token_stride, int64_t tokens, int64_t heads, int64_t topk, float scale, void* out,
+                      float* lse, void* weights, void* workspace, int64_t workspace_size, int32_t* status);
+
+/* ======================================================================
+ * slot pools that evict by accumulated attention weight
+ * ==================================================================== */
+
+/* One decode step for every request row; the counterpart of asu_lru_step with another eviction order
+ * (no reference counterpart: the reference's policies go by recency or by a hash):
+ *   1. score = decay * score, then score[last_slot[i]] += last_weight[i] for i < last_count, in that
+ *      order, each step rounded to fp32 (last_slot -1: no entry; slots without a token stay at 0);
+ *   2. while free_count < min(free_target, slot_count), the resident slot of the lowest (score,
+ *      slot) leaves among those that no key of `query` is in and whose key is below keep_from[r]
+ *      (nullable: no bound).  The slots that leave are pushed on the free stack in rising order,
+ *      their keys go to evicted[r, :n] in the same order, and evicted[r, n:min(free_target,
+ *      slot_count)] is filled with -1;
+ *   3. query[r, :] is resolved in order: a resident key is a hit, a miss pops the free stack (top
+ *      first) and starts with score 0, or is a shortage (slot -1) when the stack is empty.
+ * State per request row: token_to_slot [key_space], slot_to_token [slot_count], free_stack
+ * [slot_count], free_count as for asu_lru_step, and score [slot_count] fp32.  Outputs as for
+ * asu_lru_step.  last_slot / last_weight [last_count] per row (ASU_DTYPE_BF16 or _FP32; last_count 0:
+ * none): usually the slots of the step before and the weights that its attention gave them.
+ * slot_out may be last_slot itself when last_count == query_count.  A weight that is negative,
+ * infinite or NaN is not added and sets ASU_ST_BAD_WEIGHT; a last_slot outside [-1, slot_count)
+ * sets ASU_ST_BAD_QUERY.  Results do not depend on scheduling.
+ * Limits: slot_count <= 16384, query_count and last_count <= 4096, key_space < 2^31, decay in [0, 1]. */
+int asu_weight_step(void* stream, int32_t* token_to_slot, int32_t* slot_to_token, float* score, int32_t* free_stack,
+                    int32_t* free_count, const int32_t* last_slot, const void* last_weight, int32_t weight_dtype,
+                    uint32_t last_count, float decay, const int32_t* keep_from, const int32_t* query,
+                    int32_t* slot_out, uint8_t* hit_mask, uint8_t* install_mask, int32_t* evicted,
+                    uint32_t evicted_stride, int32_t* evicted_count, int64_t* stats, int32_t* status,
+                    uint32_t req_num, uint32_t key_space, uint32_t slot_count, uint32_t query_count,
+                    uint32_t free_target);
 
 #ifdef __cplusplus
 }
