@@ -7,7 +7,7 @@
 //
 // One CTA per (token, head); every warp takes each fourth entry, holds 16 latents and 2 rope values a
 // lane, and keeps its own running maximum and sum; the four are joined at the end.
-#include "kv4.cuh"
+#include "kv4_decode.cuh"
 
 namespace asu {
 namespace {
@@ -110,6 +110,7 @@ kv4_weights_kernel(const float* __restrict__ logits, const float* __restrict__ l
 }
 
 int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+    if (heads > 32) return wide_workspace(tokens, topk, weights);
     return weights ? tokens * heads * topk * 4 : 0;
 }
 
@@ -144,6 +145,28 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
         reinterpret_cast<uintptr_t>(workspace) % 16)
         return ASU_ERR_ALIGN;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (heads > 32) {
+        Operands op;
+        op.q = static_cast<const __nv_bfloat16*>(q);
+        op.q_token = q_token_stride;
+        op.q_head = q_head_stride;
+        op.pool = static_cast<const uint8_t*>(pool);
+        op.pool_token = pool_token_stride;
+        op.pool_pitch = pool_pitch;
+        op.pool_rows = static_cast<int32_t>(pool_rows);
+        op.slots = slots;
+        op.slots_token = slots_token_stride;
+        op.tokens = static_cast<int32_t>(tokens);
+        op.heads = static_cast<int32_t>(heads);
+        op.topk = static_cast<int32_t>(topk);
+        op.scale_log2 = scale * 1.4426950408889634f;
+        op.q_aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
+        op.out = static_cast<__nv_bfloat16*>(out);
+        op.lse = lse;
+        op.weights = static_cast<__nv_bfloat16*>(weights);
+        op.status = status;
+        return launch_wide(s, op, workspace);
+    }
     float* logits = weights != nullptr ? static_cast<float*>(workspace) : nullptr;
     int rc = launch_pdl(kv4_decode_kernel, dim3(static_cast<unsigned>(heads), static_cast<unsigned>(tokens)),
                         dim3(kThreads), 0, s, static_cast<const __nv_bfloat16*>(q), q_token_stride, q_head_stride,
