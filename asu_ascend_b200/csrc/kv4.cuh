@@ -50,5 +50,12 @@ __device__ __forceinline__ void scale_pair(uint32_t byte, __nv_bfloat162& s, __n
     c = __hmul2(s, __float2bfloat162_rn(-136.0f));
 }
 
+// The same for byte `i` of a register of scale bytes.
+__device__ __forceinline__ void scale_pair(uint32_t bytes, int i, __nv_bfloat162& s, __nv_bfloat162& c) {
+    const uint32_t both = __byte_perm(bytes, 0, 0x4040 | (i << 8) | i) * 16u + ((127 - kScaleBias) << 7) * 0x10001u;
+    s = reinterpret_cast<const __nv_bfloat162&>(both);
+    c = __hmul2(s, __float2bfloat162_rn(-136.0f));
+}
+
 }  // namespace kv4
 }  // namespace asu

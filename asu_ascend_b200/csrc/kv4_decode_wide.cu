@@ -6,39 +6,57 @@ namespace asu {
 namespace kv4 {
 namespace {
 
-// ---- many heads: tensor cores --------------------------------------------------------------------
-//
 // 128 rows of heads (padded) x 64 entries a tile.  A CTA makes 256 of the 512 output columns, since
 // all 512 in 32 bits would fill the tensor memory and leave no room for the scores; the two CTAs of a
 // token each compute the scores (1.5 times the products of a scheme that shares them, but no
 // exchange between SMs).
 //
-// Tensor memory, 512 columns: output 256, scores 2 x 64 (their weights take the same columns,
-// as bf16 pairs, once read), and q's latents 256..511, bf16 pairs, 128.
-// Shared memory, 224 KB: q's other 320 values, 80 KB; two tiles of dequantised rows, 72 KB each, as nine
-// blocks of [64 entries x 64 values] in the 128-byte swizzle.  A block serves both products: entries
+// Tensor memory, 512 columns: output 256, scores 64, their weights as bf16 pairs 32, and q's latents
+// 256..511 and rope part, bf16 pairs, 160.
+// Shared memory, 221 KB: q's latents 0..255, 64 KB; two tiles of 4-bit rows, 52 KB; and dequantised rows
+// as blocks of [64 entries x 64 values] in the 128-byte swizzle.  A block serves both products: entries
 // x values with the values contiguous is K-major for the scores and MN-major for the output.
+// "Part A", the other half's four blocks and the rope block, only the scores read; it is free again
+// when its products of this tile are done, a thousand cycles before those of the next begin, and needs
+// no second copy.  "Part B", the four blocks of this half, is held until the output product: two copies.
 //
-// 13 warps: 4 for the softmax, a thread a head (its row of scores lies in its tensor memory lane, so
-// there is no exchange); 8 that load rows, dequantise and store blocks; one whose lane 0 issues
-// the products.  The running maximum only moves when it grows by more than 2^8: until then the weights
-// stay below 2^8, exact enough in bf16 like any others, and the output needs no rescaling.
+// 15 warps: 4 for the softmax, a thread a head (its row of scores lies in its tensor memory lane, so
+// there is no exchange); 8 that dequantise; one that issues the products; two that fetch rows.  (Rows through registers instead made 8 KB of straight-line code and 5500 cycles
+// a tile: the scoreboards wait for all loads in flight, and the instruction caches did not keep up.)
+// The products of tile n's scores run while the softmax works on tile n - 1.
 //
-// The blocks that only the scores read ("part A": the other half's four and the rope block) are
-// released after them, the four output blocks ("part B") after the output product: the next tile's
-// part A is in place when the tensor cores get there, and its products hide the filling of part B.
-constexpr int kWideThreads = 13 * 32;
-constexpr int kBlock = kTile * 128;           // bytes of a [64 x 64] bf16 block
-constexpr int kQBlock = 128 * 128;            // bytes of a [128 x 64] bf16 block
+// The running maximum only moves when it grows by more than 2^8: until then the weights stay below
+// 2^8, as exact in bf16 as any others, and the output needs no rescaling.
+constexpr int kWideThreads = 15 * 32;
+constexpr int kBlock = kTile * 128;  // bytes of a [64 x 64] bf16 block
+constexpr int kQBlock = 128 * 128;   // bytes of a [128 x 64] bf16 block
+constexpr int kRawTile = kTile * kRowBytes;
 constexpr int kSmemQ = 0;
-constexpr int kSmemA = 5 * kQBlock;
-constexpr int kSmemB = kSmemA + 2 * 5 * kBlock;
-constexpr int kSmemBars = kSmemB + 2 * 4 * kBlock;
+constexpr int kSmemA = kSmemQ + 4 * kQBlock;
+constexpr int kSmemB = kSmemA + 5 * kBlock;
+constexpr int kSmemRaw = kSmemB + 2 * 4 * kBlock;
+constexpr int kSmemBars = kSmemRaw + 2 * kRawTile;
 constexpr int kWideSmem = kSmemBars + 128 + 1024;  // the base is rounded up to 1024
-constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
+constexpr uint32_t kColO = 0, kColS = 256, kColP = 320, kColQ = 352;
 constexpr float kMaxGrowth = 8.0f;
 
-enum Bar { kFullA = 0, kFullB = 2, kScores = 4, kWeights = 6, kOutput = 8, kQuery = 10, kDrain = 11, kBars = 12 };
+// Barriers.  One of a pair is that of the even tiles.  Where a waiter may be a phase behind the
+// barrier's other users there is a pair; single ones are waited for in every phase by someone that
+// the next phase depends on.
+enum Bar {
+    kRowsHere = 0,   // pair: the tile's 4-bit rows are in shared memory (64 threads' copies)
+    kRowsRead = 2,   // pair: and have been read (8 warps)
+    kFullB = 4,      // pair: part B is dequantised (8 warps)
+    kOutput = 6,     // pair: the tile's output product is done: its part B and weights are free
+    kFullA = 8,      // part A is dequantised (8 warps)
+    kFreeA = 9,      // and its products are done
+    kScores = 10,    // the tile's scores are made
+    kScoresRead = 11,  // and have been read (128 threads)
+    kWeights = 12,   // the tile's weights are in tensor memory (128 threads)
+    kQuery = 13,     // the token's q is in place (128 threads)
+    kDrain = 14,
+    kBars = 15
+};
 
 struct Scratch {
     float* ml;         // [2 * ctas][2][128] running maximum (base 2) and sum of a piece
@@ -47,23 +65,82 @@ struct Scratch {
     uint32_t* p;       // [tokens][tiles][32][128] a tile's weights, pairs of entries
 };
 
-struct RawRows {  // a thread's part of a tile before dequantising: two rows
-    uint4 code[2][2], rope[2];
-    uint32_t scale[2][2];
-};
+__device__ __forceinline__ uint4 shared_load16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t shared_load2(uint32_t at) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void shared_store16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 
-__device__ __forceinline__ void dequantise(const uint4& code, uint32_t scales, uint32_t block, int row, int lp) {
+// 32 latents as four 16-byte chunks of a swizzled row; chunk i goes to `at` with i in address bits 4 and 5.
+__device__ __forceinline__ void dequantise(const uint4& code, uint32_t scales, uint32_t at) {
     const uint32_t w[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         __nv_bfloat162 s, c;
-        scale_pair((scales >> (8 * (i / 2))) & 0xffu, s, c);
+        scale_pair(scales, i / 2, s, c);
         uint32_t v[4];
         unpack_word(w[i], s, c, v);
-        const uint32_t at = block + row * 128 + (((lp * 4 + i) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
-                     : "memory");
+        shared_store16(at ^ (i << 4), v[0], v[1], v[2], v[3]);
     }
+}
+
+// Pairs of floats in one register pair: one instruction for two.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    lo = __uint_as_float(a);
+    hi = __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// Walks the units of a CTA's range.
+struct Walk {
+    int64_t u;
+    int32_t row, tile;
+    __device__ __forceinline__ Walk(const Division& d, int64_t start) {
+        u = start;
+        row = static_cast<int32_t>(start / d.tiles);
+        tile = static_cast<int32_t>(start - static_cast<int64_t>(row) * d.tiles);
+    }
+    __device__ __forceinline__ void next(const Division& d) {
+        ++u;
+        if (++tile == d.tiles) {
+            tile = 0;
+            ++row;
+        }
+    }
+};
+
+// 8 values that start on any element.
+__device__ __noinline__ uint4 load_unaligned(const __nv_bfloat16* p, bool there) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+    if (there)
+        for (int i = 0; i < 4; ++i)
+            w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __global__ void __launch_bounds__(kWideThreads, 1)
@@ -73,252 +150,284 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
     __shared__ int s_dead;
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = base + kSmemBars;
-    auto bar = [&](int which, int64_t n) { return bars + 8u * (which + static_cast<int>(n & 1)); };
+    auto bar = [&](int which) { return bars + 8u * which; };
+    auto bar2 = [&](int which, uint32_t n) { return bars + 8u * (which + (n & 1)); };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int* dead = &s_dead;
     // by whole warps: all lanes go on, or none
     auto warp_wait = [&](uint32_t b, uint32_t parity) {
-        return __all_sync(0xffffffffu, tc::mbar_wait(b, parity, dead)) != 0;
+        return __all_sync(0xffffffffu, tc::mbar_wait(b, parity & 1, dead)) != 0;
     };
 
     if (tid == 0) {
         s_dead = 0;
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(bars + 8 * (kFullA + i), 8);
-            tc::mbar_init(bars + 8 * (kFullB + i), 8);
-            tc::mbar_init(bars + 8 * (kScores + i), 1);
-            tc::mbar_init(bars + 8 * (kWeights + i), 128);
-            tc::mbar_init(bars + 8 * (kOutput + i), 1);
+            tc::mbar_init(bar(kRowsHere + i), 64);
+            tc::mbar_init(bar(kRowsRead + i), 8);
+            tc::mbar_init(bar(kFullB + i), 8);
+            tc::mbar_init(bar(kOutput + i), 1);
         }
-        tc::mbar_init(bars + 8 * kQuery, 128);
-        tc::mbar_init(bars + 8 * kDrain, 1);
+        tc::mbar_init(bar(kFullA), 8);
+        tc::mbar_init(bar(kFreeA), 1);
+        tc::mbar_init(bar(kScores), 1);
+        tc::mbar_init(bar(kScoresRead), 128);
+        tc::mbar_init(bar(kWeights), 128);
+        tc::mbar_init(bar(kQuery), 128);
+        tc::mbar_init(bar(kDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = s_tmem;
+    // all columns are this block's: they start at 0, and the addresses below are constants
+    if (tid == 0 && s_tmem != 0) *dead = 1;
     pdl_wait();
 
     const int64_t u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
     const int tiles = div.tiles;
 
     if (warp >= 4 && warp < 12) {
-        // ---- rows: global memory -> registers -> dequantised blocks ----
-        // lane = 8 q + 2 rr + lp: row rr of four, 32 latents 32 * (2 q + lp) of either half.  Eight
-        // consecutive lanes store to four rows x two chunks, which the swizzle spreads over all banks.
+        // ---- 4-bit rows -> dequantised blocks ----
+        // lane = 8 q + 2 rr + lp: row rr of four, latents 32 * (2 q + lp) .. of either half.  Eight
+        // consecutive lanes read and store four rows x two chunks: all banks, on both sides (a row is 104
+        // words, 8 more than a multiple of 32, and the blocks are swizzled).
         const int quarter = lane >> 3, lp = lane & 1;
-        const int row0 = (warp - 4) * 4 + ((lane >> 1) & 3);
-        const int chunk = 2 * quarter + lp;
-        int32_t bits = 0;
-        int64_t row = u0 / tiles;
-        int tile = static_cast<int>(u0 - row * tiles);
-        auto slot_of = [&](int64_t r, int t, int half) -> int32_t {
-            const int e = t * kTile + half * 32 + row0;
-            if (e >= op.topk) return kNotFound;
-            const int64_t token = r % op.tokens;
-            const int32_t s = __ldg(op.slots + token * op.slots_token + e);
-            if (s >= 0 && s < op.pool_rows) return s;
-            if (s != kNotFound) bits |= ASU_ST_BAD_QUERY;
-            return kNotFound;
-        };
-        auto load = [&](RawRows& raw, int64_t r, const int32_t (&slot)[2]) {
-            const uint8_t* pool = op.pool + static_cast<uint64_t>(r % op.tokens) * op.pool_token;
+        const int row0 = (warp - 4) * 4 + ((lane >> 1) & 3);  // and row0 + 32
+        const uint32_t chunk = 2 * quarter + lp;
+        const uint32_t raw_at = base + kSmemRaw + row0 * kRowBytes;
+        const uint32_t chunk_at = quarter * kBlock + row0 * 128 + (((lp * 4) ^ (row0 & 7)) << 4);
+        const uint32_t rope_chunk = lp * 4 + quarter;
+        const uint32_t rope_at = base + kSmemA + 4 * kBlock + row0 * 128 + ((rope_chunk ^ (row0 & 7)) << 4);
+        uint32_t n = 0;
+        for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
+            const uint32_t raw = raw_at + (n & 1) * kRawTile;
+            const uint32_t mine = at.row >= op.tokens ? 8 : 0, other = 8 - mine;  // chunks before this half's
+            if (!warp_wait(bar2(kRowsHere, n), n >> 1)) break;
+            if (n >= 1 && !warp_wait(bar(kFreeA), n - 1)) break;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                raw.code[i][0] = raw.code[i][1] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-                raw.rope[i] = make_uint4(0, 0, 0, 0);
-                raw.scale[i][0] = raw.scale[i][1] = 0;
-                if (slot[i] < 0) continue;  // a row of zeros
-                const uint8_t* p = pool + static_cast<uint64_t>(slot[i]) * op.pool_pitch;
-                raw.code[i][0] = __ldg(reinterpret_cast<const uint4*>(p + chunk * 16));
-                raw.code[i][1] = __ldg(reinterpret_cast<const uint4*>(p + 128 + chunk * 16));
-                raw.scale[i][0] = __ldg(reinterpret_cast<const unsigned short*>(p + kScaleOffset + chunk * 2));
-                raw.scale[i][1] = __ldg(reinterpret_cast<const unsigned short*>(p + kScaleOffset + 16 + chunk * 2));
-                raw.rope[i] = __ldg(reinterpret_cast<const uint4*>(p + kRopeOffset + (lp * 4 + quarter) * 16));
-            }
-        };
-        RawRows cur, nxt;
-        int32_t slot[2], slot_nxt[2];
-        for (int i = 0; i < 2; ++i) slot[i] = u0 < u1 ? slot_of(row, tile, i) : kNotFound;
-        load(cur, row, slot);
-        int64_t row_n = row;
-        int tile_n = tile;
-        auto advance = [&](int64_t& r, int& t) {
-            if (++t == tiles) {
-                t = 0;
-                ++r;
-            }
-        };
-        advance(row_n, tile_n);
-        for (int i = 0; i < 2; ++i) slot_nxt[i] = u0 + 1 < u1 ? slot_of(row_n, tile_n, i) : kNotFound;
-        for (int64_t u = u0, n = 0; u < u1; ++u, ++n) {
-            // the next tile's rows and the slots of the one behind it are on their way meanwhile
-            load(nxt, row_n, slot_nxt);
-            int64_t row_nn = row_n;
-            int tile_nn = tile_n;
-            advance(row_nn, tile_nn);
-            if (u + 2 < u1)
-                for (int i = 0; i < 2; ++i) slot_nxt[i] = slot_of(row_nn, tile_nn, i);
-            else
-                slot_nxt[0] = slot_nxt[1] = kNotFound;
-            const int half = row >= op.tokens;  // this CTA's output columns: latents 256 * half ..
-            const uint32_t part_a = base + kSmemA + static_cast<int>(n & 1) * 5 * kBlock;
-            const uint32_t part_b = base + kSmemB + static_cast<int>(n & 1) * 4 * kBlock;
-            if (n >= 2 && !warp_wait(bar(kScores, n), ((n >> 1) - 1) & 1)) break;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = row0 + 32 * i;
-                const uint4 c = half ? cur.code[i][0] : cur.code[i][1];
-                dequantise(c, half ? cur.scale[i][0] : cur.scale[i][1], part_a + quarter * kBlock, r, lp);
-                const uint32_t at = part_a + 4 * kBlock + r * 128 + (((lp * 4 + quarter) ^ (r & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(cur.rope[i].x),
-                             "r"(cur.rope[i].y), "r"(cur.rope[i].z), "r"(cur.rope[i].w)
-                             : "memory");
+                const uint32_t from = raw + i * 32 * kRowBytes;
+                const uint4 code = shared_load16(from + (other + chunk) * 16);
+                const uint32_t scales = shared_load2(from + kScaleOffset + (other + chunk) * 2);
+                const uint4 rope = shared_load16(from + kRopeOffset + rope_chunk * 16);
+                shared_store16(rope_at + i * 32 * 128, rope.x, rope.y, rope.z, rope.w);
+                dequantise(code, scales, base + kSmemA + chunk_at + i * 32 * 128);
             }
             tc::fence_async_shared();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(bar(kFullA, n));
-            if (n >= 2 && !warp_wait(bar(kOutput, n), ((n >> 1) - 1) & 1)) break;
+            if (lane == 0) tc::mbar_arrive(bar(kFullA));
+            if (n >= 2 && !warp_wait(bar2(kOutput, n), (n >> 1) - 1)) break;
+            const uint32_t part_b = base + kSmemB + (n & 1) * 4 * kBlock;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint4 c = half ? cur.code[i][1] : cur.code[i][0];
-                dequantise(c, half ? cur.scale[i][1] : cur.scale[i][0], part_b + quarter * kBlock, row0 + 32 * i, lp);
+                const uint32_t from = raw + i * 32 * kRowBytes;
+                const uint4 code = shared_load16(from + (mine + chunk) * 16);
+                const uint32_t scales = shared_load2(from + kScaleOffset + (mine + chunk) * 2);
+                dequantise(code, scales, part_b + chunk_at + i * 32 * 128);
             }
             tc::fence_async_shared();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(bar(kFullB, n));
-            cur = nxt;
-            row = row_n;
-            tile = tile_n;
-            row_n = row_nn;
-            tile_n = tile_nn;
+            if (lane == 0) {
+                tc::mbar_arrive(bar2(kFullB, n));
+                tc::mbar_arrive(bar2(kRowsRead, n));
+            }
         }
+    } else if (warp >= 13) {
+        // ---- rows: asynchronous copies, two tiles ahead; slots three.  32 rows of a tile a warp, 26 lanes a
+        // row.  (One bulk copy a row took 40 ns each and was the bound.) ----
+        const int row0 = (warp - 13) * 32;
+        int32_t bits = 0;
+        auto slot_of = [&](const Walk& w) -> int32_t {
+            const int e = w.tile * kTile + row0 + lane;
+            if (w.u >= u1 || e >= op.topk) return kNotFound;
+            return __ldg(op.slots + (w.row < op.tokens ? w.row : w.row - op.tokens) * op.slots_token + e);
+        };
+        Walk at(div, u0);
+        int32_t slot = slot_of(at);
+        const uint32_t raw_at = base + kSmemRaw + row0 * kRowBytes + lane * 16;
+        for (uint32_t n = 0; at.u < u1; ++n) {
+            // an entry that is not there copies nothing and leaves zeros: finite values, whose weights are 0
+            const bool there = slot >= 0 && slot < op.pool_rows;
+            if (!there && slot != kNotFound) bits |= ASU_ST_BAD_QUERY;
+            const uint64_t from = reinterpret_cast<uint64_t>(op.pool) +
+                                  static_cast<uint64_t>(at.row < op.tokens ? at.row : at.row - op.tokens) * op.pool_token +
+                                  static_cast<uint64_t>(there ? slot : 0) * op.pool_pitch;
+            const uint32_t valid = __ballot_sync(0xffffffffu, there);
+            at.next(div);
+            slot = slot_of(at);
+            if (n >= 2 && !warp_wait(bar2(kRowsRead, n), (n >> 1) - 1)) break;
+            const uint32_t to = raw_at + (n & 1) * kRawTile;
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+                const uint64_t src = __shfl_sync(0xffffffffu, from, r) + lane * 16;
+                if (lane < kRowBytes / 16)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * kRowBytes), "l"(src),
+                                 "r"((valid >> r) & 1u ? 16 : 0)
+                                 : "memory");
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar2(kRowsHere, n)) : "memory");
+        }
+        // no copy may land after this block has ended, whatever way the loops were left
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (bits) flag_status(op.status, 0, bits);
     } else if (warp == 12) {
-        if (lane == 0) {
-            // ---- the products ----
-            constexpr uint32_t kDescS = tc::instruction(128, kTile, false);
-            constexpr uint32_t kDescO = tc::instruction(128, 256, true);
-            auto scores = [&](int64_t n, int half) {
-                const uint32_t part_a = base + kSmemA + static_cast<int>(n & 1) * 5 * kBlock;
-                const uint32_t part_b = base + kSmemB + static_cast<int>(n & 1) * 4 * kBlock;
-                const uint32_t d = tmem + kColS + kTile * static_cast<uint32_t>(n & 1);
-                // of the two halves of the latents, q's first lies in shared and its second in tensor memory
-                auto block = [&](uint32_t rows, int which, uint32_t accumulate) {  // which: 64 values of q
+        // ---- the products: the whole warp keeps step, one lane issues ----
+        constexpr uint32_t kDescS = tc::instruction(128, kTile, false);
+        constexpr uint32_t kDescO = tc::instruction(128, 256, true);
+        const uint32_t desc_q = tc::operand(base + kSmemQ, 0);
+        const uint32_t desc_a = tc::operand(base + kSmemA, 0);
+        const uint32_t desc_b = tc::operand(base + kSmemB, 0);
+        const uint32_t desc_v = tc::operand(base + kSmemB, kBlock);
+        // four blocks of latents with q's 0..255 (shared memory) or 256..511 (tensor memory)
+        auto low = [&](uint32_t rows) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint64_t b = tc::operand(rows + k * 32, 0, 1024);
-                        if (which >= 4 && which < 8) {
-                            tc::mma_ts(d, tmem + kColQ + (which - 4) * 32 + k * 8, b, kDescS, accumulate | (k > 0));
-                        } else {
-                            const uint32_t q = base + kSmemQ + (which < 4 ? which : 4) * kQBlock + k * 32;
-                            tc::mma_ss(d, tc::operand(q, 0, 1024), b, kDescS, accumulate | (k > 0));
-                        }
-                    }
-                };
-                if (!tc::mbar_wait(bar(kFullA, n), (n >> 1) & 1, dead)) return false;
-                tc::fence_after();
-                block(part_a + 4 * kBlock, 8, 0);
-                for (int i = 0; i < 4; ++i) block(part_a + i * kBlock, (half ? 0 : 4) + i, 1);
-                if (!tc::mbar_wait(bar(kFullB, n), (n >> 1) & 1, dead)) return false;
-                tc::fence_after();
-                for (int i = 0; i < 4; ++i) block(part_b + i * kBlock, (half ? 4 : 0) + i, 1);
-                tc::commit(bar(kScores, n));
-                return true;
-            };
-            int64_t n = 0, segment = 0;
-            bool ok = true;
-            for (int64_t u = u0; ok && u < u1; ++u, ++n) {
-                const int64_t row = u / tiles;
-                const int half = row >= op.tokens;
-                const bool first = u == u0 || u == row * tiles;
-                const bool last = u + 1 == u1 || u + 1 == (row + 1) * tiles;
-                if (first) {
-                    ok = tc::mbar_wait(bars + 8 * kQuery, segment & 1, dead);
-                    ++segment;
-                    if (!ok) break;
-                    tc::fence_after();
-                    if (!(ok = scores(n, half))) break;
-                }
-                if (!last) {
-                    // the other score columns hold the weights of tile n - 1 until its output product is done
-                    if (!first && !(ok = tc::mbar_wait(bar(kOutput, n - 1), ((n - 1) >> 1) & 1, dead))) break;
-                    tc::fence_after();
-                    if (!(ok = scores(n + 1, half))) break;
-                }
-                if (!(ok = tc::mbar_wait(bar(kWeights, n), (n >> 1) & 1, dead))) break;
-                tc::fence_after();
-                const uint32_t part_b = base + kSmemB + static_cast<int>(n & 1) * 4 * kBlock;
-                const uint32_t p = tmem + kColS + kTile * static_cast<uint32_t>(n & 1);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    tc::mma_ss(kColS, desc_q + i * (kQBlock / 16) + 2 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+        };
+        auto high = [&](uint32_t rows) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    tc::mma_ts(kColS, kColQ + i * 32 + 8 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+        };
+        auto rope = [&] {  // the first product of a tile's scores
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                tc::mma_ts(kColS, kColQ + 4 * 32 + 8 * k, desc_a + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
+        };
+        auto scores = [&](uint32_t n, int half) {
+            if (n >= 1 && !warp_wait(bar(kScoresRead), n - 1)) return false;
+            if (!warp_wait(bar(kFullA), n)) return false;
+            tc::fence_after();
+            if (tc::elect_one()) {
+                rope();
+                if (half) low(desc_a);
+                else high(desc_a);
+                tc::commit(bar(kFreeA));
+            }
+            __syncwarp();
+            if (!warp_wait(bar2(kFullB, n), n >> 1)) return false;
+            tc::fence_after();
+            if (tc::elect_one()) {
+                const uint32_t rows = desc_b + (n & 1) * (4 * kBlock / 16);
+                if (half) high(rows);
+                else low(rows);
+                tc::commit(bar(kScores));
+            }
+            __syncwarp();
+            return true;
+        };
+        auto output = [&](uint32_t n, bool accumulate) {
+            if (!warp_wait(bar(kWeights), n)) return false;
+            tc::fence_after();
+            if (tc::elect_one()) {
+                const uint32_t v = desc_v + (n & 1) * (4 * kBlock / 16);
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                    tc::mma_ts(tmem + kColO, p + 8 * k, tc::operand(part_b + k * 2048, kBlock, 1024), kDescO,
-                               !first || k > 0);
-                tc::commit(bar(kOutput, n));
+                    tc::mma_ts(kColO, kColP + 8 * k, v + k * (2048 / 16), kDescO, accumulate || k > 0);
+                tc::commit(bar2(kOutput, n));
             }
-            if (!ok) {  // nothing of this block may still run when its tensor memory is given back
-                tc::commit(bars + 8 * kDrain);
-                for (int i = 0; i < tc::kSpinLimit && !tc::mbar_try(bars + 8 * kDrain, 0); ++i) {
-                }
+            __syncwarp();
+            return true;
+        };
+        uint32_t n = 0, segment = 0;
+        bool before_first = true;  // was tile n - 1 the first of its piece?
+        for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
+            const bool first = at.u == u0 || at.tile == 0;
+            if (first) {
+                // the token before is finished first: its weights do not depend on this one's q
+                if (n > 0 && !output(n - 1, !before_first)) break;
+                if (!warp_wait(bar(kQuery), segment)) break;
+                ++segment;
             }
+            if (!scores(n, at.row >= op.tokens)) break;
+            if (!first && !output(n - 1, !before_first)) break;
+            before_first = first;
+            if (at.u + 1 == u1 && !output(n, !first)) break;
         }
-        __syncwarp();
     } else {
         // ---- softmax, a thread a head ----
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         const int head = tid;
-        float m = -INFINITY, l = 0.0f;
-        int64_t n = 0;
-        for (int64_t u = u0; u < u1; ++u, ++n) {
-            const int64_t row = u / tiles;
-            const int half = row >= op.tokens;
-            const int64_t token = row - (half ? op.tokens : 0);
-            const int tile = static_cast<int>(u - row * tiles);
-            const bool first = u == u0 || tile == 0;
-            const bool last = u + 1 == u1 || tile + 1 == tiles;
-            if (first) {
-                // this token's q: latents 0..255 and the rope part to shared memory, the rest to tensor memory
-                const __nv_bfloat16* qt = op.q + token * op.q_token;
-                auto chunk8 = [&](int h, int at) -> uint4 {
-                    if (h >= op.heads) return make_uint4(0, 0, 0, 0);
-                    const __nv_bfloat16* p = qt + h * op.q_head + at;
-                    if (op.q_aligned) return __ldg(reinterpret_cast<const uint4*>(p));
-                    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-                    uint32_t w[4];
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
-                    return make_uint4(w[0], w[1], w[2], w[3]);
-                };
-#pragma unroll 8
-                for (int i = tid; i < 5 * 128 * 8; i += 128) {
-                    const int block = i >> 10, h = (i >> 3) & 127, c = i & 7;
-                    const uint4 v = chunk8(h, (block < 4 ? block * 64 : kLatent) + c * 8);
-                    const uint32_t at = base + kSmemQ + block * kQBlock + h * 128 + ((c ^ (h & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
-                                 "r"(v.w)
-                                 : "memory");
-                }
-                tc::fence_async_shared();
+        // A token's q, zero for heads beyond the last: latents 0..255 to shared memory (asynchronous
+        // copies), the rest to tensor memory.  Every score of the token before must have been made.
+        auto load_q = [&](int32_t token) {
+            const __nv_bfloat16* q = op.q + token * op.q_token;
+            const int c = tid & 7;
+#pragma unroll 1
+            for (int h = tid >> 3; h < 128; h += 16) {
+                const bool there = h < op.heads;
+                const __nv_bfloat16* from = q + (there ? h : 0) * op.q_head + c * 8;
+                const uint32_t to = base + kSmemQ + h * 128 + ((c ^ (h & 7)) << 4);
+                if (op.q_aligned) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint4 v = chunk8(head, 256 + i * 64 + k * 8);
-                        w[4 * k] = v.x;
-                        w[4 * k + 1] = v.y;
-                        w[4 * k + 2] = v.z;
-                        w[4 * k + 3] = v.w;
+                    for (int k = 0; k < 4; ++k)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * kQBlock),
+                                     "l"(from + k * 64), "r"(there ? 16 : 0)
+                                     : "memory");
+                } else {
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 v = load_unaligned(from + k * 64, there);
+                        shared_store16(to + k * kQBlock, v.x, v.y, v.z, v.w);
                     }
-                    tc::tmem_store32(lanes + kColQ + i * 32, w);
                 }
-                tc::tmem_wait_store();
-                tc::fence_before();
-                tc::mbar_arrive(bars + 8 * kQuery);
+            }
+            const bool there = head < op.heads;
+            const __nv_bfloat16* mine = q + (there ? head : 0) * op.q_head + 256;
+            uint4 w[2][8];  // one group of 64 values is on its way while the one before is stored
+            auto fetch = [&](int i, uint4 (&v)[8]) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const __nv_bfloat16* from = mine + i * 64 + k * 8;
+                    v[k] = op.q_aligned ? __ldg(reinterpret_cast<const uint4*>(from)) : load_unaligned(from, there);
+                }
+            };
+            fetch(0, w[0]);
+#pragma unroll
+            for (int i = 0; i < 5; ++i) {
+                if (i < 4) fetch(i + 1, w[(i + 1) & 1]);
+                uint32_t x[32];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[4 * k] = there ? w[i & 1][k].x : 0u;
+                    x[4 * k + 1] = there ? w[i & 1][k].y : 0u;
+                    x[4 * k + 2] = there ? w[i & 1][k].z : 0u;
+                    x[4 * k + 3] = there ? w[i & 1][k].w : 0u;
+                }
+                __syncwarp();
+                tc::tmem_store32(lanes + kColQ + i * 32, x);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc::fence_async_shared();
+            tc::tmem_wait_store();
+            tc::fence_before();
+            tc::mbar_arrive(bar(kQuery));
+        };
+        float m = -INFINITY;
+        uint64_t l2 = 0;  // the sum of the even and of the odd entries
+        Walk at(div, u0);
+        load_q(at.row < op.tokens ? at.row : at.row - op.tokens);
+        for (uint32_t n = 0; at.u < u1; at.next(div), ++n) {
+            const int half = at.row >= op.tokens;
+            const int64_t token = at.row - (half ? op.tokens : 0);
+            const int tile = at.tile;
+            const bool first = at.u == u0 || tile == 0;
+            const bool last = at.u + 1 == u1 || tile + 1 == tiles;
+            if (first) {
                 m = -INFINITY;
-                l = 0.0f;
+                l2 = 0;
+                // the next token's q to L2: its loads come between two tokens, where nothing hides them
+                const int64_t next = static_cast<int64_t>(at.row + 1) * tiles;
+                if (next < u1 && head < op.heads) {
+                    const __nv_bfloat16* q =
+                        op.q + (at.row + 1 < op.tokens ? at.row + 1 : at.row + 1 - op.tokens) * op.q_token + head * op.q_head;
+#pragma unroll
+                    for (int k = 0; k < kDim; k += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k));
+                }
             }
             // which entries are there
             uint32_t there[2];
@@ -328,14 +437,15 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 const int32_t s = e < op.topk ? __ldg(op.slots + token * op.slots_token + e) : kNotFound;
                 there[i] = __ballot_sync(0xffffffffu, s >= 0 && s < op.pool_rows);
             }
-            if (!warp_wait(bar(kScores, n), (n >> 1) & 1)) break;
+            if (!warp_wait(bar(kScores), n)) break;
             tc::fence_after();
-            const uint32_t cols = lanes + kColS + kTile * static_cast<uint32_t>(n & 1);
             uint32_t s[2][32];
-            tc::tmem_load32(cols, s[0]);
-            tc::tmem_load32(cols + 32, s[1]);
+            tc::tmem_load32(lanes + kColS, s[0]);
+            tc::tmem_load32(lanes + kColS + 32, s[1]);
             tc::tmem_wait_load(s[0]);
             tc::tmem_wait_load(s[1]);
+            tc::fence_before();
+            tc::mbar_arrive(bar(kScoresRead));
             if ((there[0] & there[1]) != 0xffffffffu) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
@@ -352,10 +462,14 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 fade = exp2_fast(m - top);
                 m = top;
             }
+            const float from = m == -INFINITY ? 0.0f : m;
+            // the output product before has read the weights there
+            if (n >= 1 && !warp_wait(bar2(kOutput, n - 1), (n - 1) >> 1)) break;
+            tc::fence_after();
             if (__any_sync(0xffffffffu, fade != 1.0f)) {
-                l *= fade;
-                if (!warp_wait(bar(kOutput, n - 1), ((n - 1) >> 1) & 1)) break;
-                tc::fence_after();
+                float a, b;
+                unpair(l2, a, b);
+                l2 = pair(__float_as_uint(a * fade), __float_as_uint(b * fade));
 #pragma unroll 1
                 for (int c = 0; c < 256; c += 32) {
                     uint32_t o[32];
@@ -365,32 +479,40 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                     for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fade);
                     tc::tmem_store32(lanes + kColO + c, o);
                 }
-                tc::tmem_wait_store();
             }
-            const float from = m == -INFINITY ? 0.0f : m;
+            const uint64_t scale2 = pair(__float_as_uint(op.scale_log2), __float_as_uint(op.scale_log2));
+            const uint64_t from2 = pair(__float_as_uint(-from), __float_as_uint(-from));
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const float a = exp2_fast(fmaf(__uint_as_float(s[i / 16][(2 * i) % 32]), op.scale_log2, -from));
-                const float b = exp2_fast(fmaf(__uint_as_float(s[i / 16][(2 * i + 1) % 32]), op.scale_log2, -from));
-                l += a;
-                l += b;
+                float a, b;
+                unpair(fma2(pair(s[i / 16][(2 * i) % 32], s[i / 16][(2 * i + 1) % 32]), scale2, from2), a, b);
+                a = exp2_fast(a);
+                b = exp2_fast(b);
+                l2 = add2(l2, pair(__float_as_uint(a), __float_as_uint(b)));
                 p[i] = pack_bf16(a, b);
             }
-            tc::tmem_store32(cols, p);
+            tc::tmem_store32(lanes + kColP, p);
             tc::tmem_wait_store();
             tc::fence_before();
-            tc::mbar_arrive(bar(kWeights, n));
+            tc::mbar_arrive(bar(kWeights));
             if (op.weights != nullptr && half == 0) {
-                const int64_t at = token * tiles + tile;
-                scratch.ref[at * 128 + head] = m;
+                const int64_t to = token * tiles + tile;
+                scratch.ref[to * 128 + head] = m;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) scratch.p[(at * 32 + i) * 128 + head] = p[i];
+                for (int i = 0; i < 32; ++i) scratch.p[(to * 32 + i) * 128 + head] = p[i];
             }
             if (last) {
-                if (!warp_wait(bar(kOutput, n), (n >> 1) & 1)) break;
+                // this token's scores are all made: the next one's q, whose first scores then run
+                // beside what follows here
+                if (at.u + 1 < u1) load_q(at.row + 1 < op.tokens ? at.row + 1 : at.row + 1 - op.tokens);
+                float l, odd;
+                unpair(l2, l, odd);
+                l += odd;
+                if (!warp_wait(bar2(kOutput, n), n >> 1)) break;
                 tc::fence_after();
-                const bool whole = row * tiles >= u0 && (row + 1) * tiles <= u1;
+                const int64_t row_start = static_cast<int64_t>(at.row) * tiles;
+                const bool whole = row_start >= u0 && row_start + tiles <= u1;
                 if (whole) {
                     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                     __nv_bfloat16* out = op.out + (token * op.heads + head) * kLatent + half * 256;
@@ -410,12 +532,13 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                                 reinterpret_cast<uint4*>(out + c)[i] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
+                        __syncwarp();
                     }
                     if (half == 0 && head < op.heads)
                         op.lse[token * op.heads + head] =
                             l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
                 } else {
-                    const int piece = div.piece(blockIdx.x, row * tiles);
+                    const int piece = div.piece(blockIdx.x, row_start);
                     float* to = scratch.o + static_cast<int64_t>(piece) * 256 * 128 + head;
 #pragma unroll 1
                     for (int c = 0; c < 256; c += 32) {
@@ -436,77 +559,99 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
     __syncthreads();
     if (s_dead && tid == 0) flag_status(op.status, 0, ASU_ST_TIMEOUT);
     if (warp == 12) {
+        // Nothing of this block may be in flight when its tensor memory goes and its barriers with it,
+        // whatever way the loops were left.
+        if (tc::elect_one()) {
+            tc::commit(bar(kDrain));
+            for (int i = 0; i < tc::kSpinLimit && !tc::mbar_try(bar(kDrain), 0); ++i) {
+            }
+        }
+        __syncwarp();
         tc::fence_after();
-        tc::tmem_free<512>(tmem);
+        tc::tmem_free<512>(s_tmem);
     }
 }
 
 // Joins the pieces of the rows that several CTAs share, and sums the weights over the heads.
-//   blocks y < 16: output columns [16 * y, ...) ... of the token's two halves
+//   blocks y < 64: 8 output columns of one half of a token; a thread takes a head's 8 columns of every
+//                  kGroups-th piece, the groups are added up in shared memory in their order
 //   other blocks:  one tile's weights: weights_j = sum_h p_hj 2^(ref_h - lse_h)
-constexpr int kFinishThreads = 256;
-__global__ void __launch_bounds__(kFinishThreads)
+template <int kGroups>
+__global__ void __launch_bounds__(128 * kGroups)
 kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scratch) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_tile[32][129];
-    __shared__ float s_lse[128];  // base 2
+    __shared__ float s_sum[kGroups][10][128];  // 8 columns, sum of exponentials, maximum
     const int64_t token = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool joins = blockIdx.y < 16;
-    const int half = joins ? blockIdx.y >> 3 : 0;
+    const int head = tid & 127, group = tid >> 7;
+    const bool joins = blockIdx.y < 64;
+    const int half = joins ? blockIdx.y >> 5 : 0;
     const int64_t first = (half * static_cast<int64_t>(op.tokens) + token) * div.tiles;
     const int i0 = div.cta_of(first), i1 = div.cta_of(first + div.tiles - 1);
     if (joins && i0 == i1) return;  // written by its one CTA
-    if (joins) {
-        const int c0 = (blockIdx.y & 7) * 32;
-        const int head = tid & 127, part = tid >> 7;  // two threads a head, 16 columns each
-        float m = -INFINITY;
-        for (int i = i0; i <= i1; ++i) m = fmaxf(m, scratch.ml[div.piece(i, first) * 256 + head]);
-        float l = 0.0f, acc[16] = {};
-        for (int i = i0; i <= i1; ++i) {
+    float m = -INFINITY, l = 0.0f;  // of the token's head, maximum in base 2
+    if (i0 != i1) {
+        for (int i = i0 + group; i <= i1; i += kGroups) m = fmaxf(m, scratch.ml[div.piece(i, first) * 256 + head]);
+        s_sum[group][9][head] = m;
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s_sum[g][9][head]);
+        float acc[8] = {};
+        const int c0 = (blockIdx.y & 31) * 8;
+#pragma unroll 2
+        for (int i = i0 + group; i <= i1; i += kGroups) {
             const int piece = div.piece(i, first);
             const float pm = scratch.ml[piece * 256 + head];
             const float f = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
             l += scratch.ml[piece * 256 + 128 + head] * f;
-            const float* o = scratch.o + (static_cast<int64_t>(piece) * 256 + c0 + part * 16) * 128 + head;
+            if (joins) {
+                const float* o = scratch.o + (static_cast<int64_t>(piece) * 256 + c0) * 128 + head;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) acc[c] += o[c * 128] * f;
-        }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) s_tile[part * 16 + c][head] = acc[c] * inv;
-        if (blockIdx.y == 0 && part == 0 && head < op.heads)
-            op.lse[token * op.heads + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-        __syncthreads();
-        for (int i = tid; i < op.heads * 16; i += kFinishThreads) {
-            const int h = i >> 4, c = (i & 15) * 2;
-            *reinterpret_cast<uint32_t*>(op.out + (token * op.heads + h) * kLatent + half * 256 + c0 + c) =
-                pack_bf16(s_tile[c][h], s_tile[c + 1][h]);
-        }
-        return;
-    }
-    // the token's lse again (the joining blocks may not have written it yet)
-    if (tid < 128) {
-        float v = -INFINITY;
-        if (tid < op.heads) {
-            if (i0 == i1) {
-                v = op.lse[token * op.heads + tid] * 1.4426950408889634f;
-            } else {
-                float m = -INFINITY, l = 0.0f;
-                for (int i = i0; i <= i1; ++i) m = fmaxf(m, scratch.ml[div.piece(i, first) * 256 + tid]);
-                for (int i = i0; i <= i1; ++i) {
-                    const int piece = div.piece(i, first);
-                    const float pm = scratch.ml[piece * 256 + tid];
-                    l += scratch.ml[piece * 256 + 128 + tid] * (pm == -INFINITY ? 0.0f : exp2_fast(pm - m));
-                }
-                if (l > 0.0f) v = m + log2f(l);
+                for (int c = 0; c < 8; ++c) acc[c] += o[c * 128] * f;
             }
         }
-        s_lse[tid] = v;
+        s_sum[group][8][head] = l;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) s_sum[group][c][head] = acc[c];
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) l += s_sum[g][8][head];
+        if (joins) {
+            if (group == 0 && head < op.heads) {
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                uint32_t w[4];
+#pragma unroll
+                for (int c = 0; c < 8; c += 2) {
+                    float a = 0.0f, b = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        a += s_sum[g][c][head];
+                        b += s_sum[g][c + 1][head];
+                    }
+                    w[c / 2] = pack_bf16(a * inv, b * inv);
+                }
+                *reinterpret_cast<uint4*>(op.out + (token * op.heads + head) * kLatent + half * 256 + c0) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+                if (blockIdx.y == 0)
+                    op.lse[token * op.heads + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            }
+            return;
+        }
+        __syncthreads();
+    }
+    float* s_lse = s_sum[0][0];  // base 2
+    if (group == 0) {
+        float v = -INFINITY;
+        if (head < op.heads) {
+            if (i0 != i1) v = l > 0.0f ? m + log2f(l) : -INFINITY;
+            else v = op.lse[token * op.heads + head] * 1.4426950408889634f;
+        }
+        s_lse[head] = v;
     }
     __syncthreads();
-    const int tile = blockIdx.y - 16;
+    const int tile = blockIdx.y - 64;
     const int64_t at = token * div.tiles + tile;
     float f[4];
 #pragma unroll
@@ -514,7 +659,8 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
         const int h = lane * 4 + i;
         f[i] = s_lse[h] == -INFINITY ? 0.0f : exp2_fast(scratch.ref[at * 128 + h] - s_lse[h]);
     }
-    for (int k = warp; k < 32; k += kFinishThreads / 32) {  // a warp a pair of entries
+#pragma unroll 4
+    for (int k = warp; k < 32; k += 4 * kGroups) {  // a warp a pair of entries
         const uint4 p = *reinterpret_cast<const uint4*>(scratch.p + (at * 32 + k) * 128 + lane * 4);
         const uint32_t w[4] = {p.x, p.y, p.z, p.w};
         float a = 0.0f, b = 0.0f;
@@ -574,12 +720,13 @@ int launch_wide(cudaStream_t s, const Operands& op, void* workspace) {
     if (rc != ASU_OK) return rc;
     if (max_dynamic < kWideSmem) return ASU_ERR_ARG;
     rc = launch_pdl(kv4_decode_wide_kernel, dim3(d.ctas), dim3(kWideThreads), kWideSmem, s, op, d, scratch);
-    bool shared_rows = false;  // does any row lie in several CTAs' ranges?
-    for (int i = 1; i < d.ctas && !shared_rows; ++i) shared_rows = d.start(i) % d.tiles != 0;
-    if (rc != ASU_OK || (!shared_rows && op.weights == nullptr)) return rc;
-    return launch_pdl(kv4_finish_wide_kernel,
-                      dim3(static_cast<unsigned>(op.tokens), 16 + (op.weights != nullptr ? d.tiles : 0)),
-                      dim3(kFinishThreads), 0, s, op, d, scratch);
+    int most = 1;  // pieces of a row
+    for (int i = 1; i < d.ctas && most < 3; ++i)
+        if (d.start(i) % d.tiles != 0) most = d.start(i + 1) / d.tiles == d.start(i) / d.tiles && i + 1 < d.ctas ? 3 : 2;
+    if (rc != ASU_OK || (most == 1 && op.weights == nullptr)) return rc;
+    const dim3 grid(static_cast<unsigned>(op.tokens), 64 + (op.weights != nullptr ? d.tiles : 0));
+    if (most > 2) return launch_pdl(kv4_finish_wide_kernel<8>, grid, dim3(1024), 0, s, op, d, scratch);
+    return launch_pdl(kv4_finish_wide_kernel<2>, grid, dim3(256), 0, s, op, d, scratch);
 }
 
 }  // namespace kv4

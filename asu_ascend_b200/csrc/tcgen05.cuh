@@ -38,6 +38,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+    return one != 0;
+}
+
 // Generic stores to shared memory become visible to the tensor cores' (async) proxy.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -93,10 +100,13 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 //   K-major (rows are M or N, 64 elements of K a row): `stride` between 8-row groups, `lead` unused.
 //   MN-major (rows are K, 64 elements of M or N a row): `lead` between 64-element blocks of M or N,
 //   `stride` between groups of 8 K.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(lead >> 4) << 16) |
-           (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Its descriptor's lower half holds the address (units of 16 bytes; advancing within the operand is an
+// addition), the upper half depends on the layout alone and is an immediate of the products below: with
+// both halves in ordinary registers the moves to uniform ones took longer than the products.
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
+    return ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);
 }
+constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024
 
 // kind::f16: bf16 x bf16 -> fp32, M x N, K = 16.
 __host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_mn_major) {
@@ -104,18 +114,21 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_mn_major
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{ .reg .pred p; .reg .b64 x, y; setp.ne.u32 p, %4, 0;\n"
+        "mov.b64 x, {%1, %5}; mov.b64 y, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A from tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{ .reg .pred p; .reg .b64 y; setp.ne.u32 p, %4, 0;\n"
+        "mov.b64 y, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh)
         : "memory");
 }
 // The barrier completes when every tcgen05.mma issued by this thread so far has.
