@@ -27,19 +27,46 @@ struct Operands {
 };
 
 // Row (token of one part of the call) r has `tiles` consecutive units; CTA i takes the units
-// [start(i), start(i + 1)), which differ by one at most.  A row that lies in several CTAs' ranges is
-// joined afterwards.  The division depends on the call's sizes alone, so results repeat.
+// [start(i), start(i + 1)), `each` of them and one more in the first `more` CTAs.  A row that lies in
+// several CTAs' ranges is joined afterwards.  The division depends on the call's sizes alone, so results
+// repeat.  All in 32 bits: 64-bit divisions were a third of the kernels' code.
 struct Division {
-    int32_t rows, tiles, ctas;
-    __host__ __device__ __forceinline__ int64_t units() const { return static_cast<int64_t>(rows) * tiles; }
-    __host__ __device__ __forceinline__ int64_t start(int i) const { return units() * i / ctas; }
-    __host__ __device__ __forceinline__ int cta_of(int64_t u) const {
-        return static_cast<int>(((u + 1) * ctas - 1) / units());
+    int32_t rows, tiles, ctas, each, more;
+    Division() = default;
+    Division(int64_t rows_, int64_t tiles_, int64_t most) {
+        rows = static_cast<int32_t>(rows_);
+        tiles = static_cast<int32_t>(tiles_);
+        const int64_t units = rows_ * tiles_;  // below 2^26: tokens, entries and parts are bounded
+        ctas = static_cast<int32_t>(units < most ? units : most);
+        each = static_cast<int32_t>(units / ctas);
+        more = static_cast<int32_t>(units % ctas);
+    }
+    __host__ __device__ __forceinline__ int32_t start(int32_t i) const { return i * each + (i < more ? i : more); }
+    __host__ __device__ __forceinline__ int32_t cta_of(int32_t u) const {
+        const int32_t first = more * (each + 1);
+        return u < first ? u / (each + 1) : more + (u - first) / each;
     }
     // Scratch slot of CTA i's piece of a row that starts at unit `row_start`: a CTA's range holds at
     // most two pieces of rows, one at its start and one at its end.
-    __host__ __device__ __forceinline__ int piece(int i, int64_t row_start) const {
+    __host__ __device__ __forceinline__ int32_t piece(int32_t i, int32_t row_start) const {
         return 2 * i + (start(i) >= row_start ? 0 : 1);
+    }
+};
+
+// Walks the units of a CTA's range.
+struct Walk {
+    int32_t u, row, tile;
+    __device__ __forceinline__ Walk(const Division& d, int32_t start) {
+        u = start;
+        row = start / d.tiles;
+        tile = start - row * d.tiles;
+    }
+    __device__ __forceinline__ void next(const Division& d) {
+        ++u;
+        if (++tile == d.tiles) {
+            tile = 0;
+            ++row;
+        }
     }
 };
 

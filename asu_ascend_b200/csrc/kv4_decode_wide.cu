@@ -115,31 +115,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-// Walks the units of a CTA's range.
-struct Walk {
-    int64_t u;
-    int32_t row, tile;
-    __device__ __forceinline__ Walk(const Division& d, int64_t start) {
-        u = start;
-        row = static_cast<int32_t>(start / d.tiles);
-        tile = static_cast<int32_t>(start - static_cast<int64_t>(row) * d.tiles);
-    }
-    __device__ __forceinline__ void next(const Division& d) {
-        ++u;
-        if (++tile == d.tiles) {
-            tile = 0;
-            ++row;
-        }
-    }
-};
-
 // 8 values that start on any element.
-__device__ __noinline__ uint4 load_unaligned(const __nv_bfloat16* p, bool there) {
-    uint32_t w[4] = {0, 0, 0, 0};
+__device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
+    uint32_t w[4];
     const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-    if (there)
-        for (int i = 0; i < 4; ++i)
-            w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -184,7 +166,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
     if (tid == 0 && s_tmem != 0) *dead = 1;
     pdl_wait();
 
-    const int64_t u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
+    const int32_t u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
     const int tiles = div.tiles;
 
     if (warp >= 4 && warp < 12) {
@@ -272,136 +254,143 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (bits) flag_status(op.status, 0, bits);
     } else if (warp == 12) {
-        // ---- the products: the whole warp keeps step, one lane issues ----
-        constexpr uint32_t kDescS = tc::instruction(128, kTile, false);
-        constexpr uint32_t kDescO = tc::instruction(128, 256, true);
-        const uint32_t desc_q = tc::operand(base + kSmemQ, 0);
-        const uint32_t desc_a = tc::operand(base + kSmemA, 0);
-        const uint32_t desc_b = tc::operand(base + kSmemB, 0);
-        const uint32_t desc_v = tc::operand(base + kSmemB, kBlock);
-        // four blocks of latents with q's 0..255 (shared memory) or 256..511 (tensor memory)
-        auto low = [&](uint32_t rows) {
+        // ---- the products, all by one lane.  (The branch has to be that of elect.sync itself: with a plain
+        // lane number, or its result kept, the issue of a product takes 80 cycles instead of 30.) ----
+        if (tc::elect_one()) {
+            constexpr uint32_t kDescS = tc::instruction(128, kTile, false);
+            constexpr uint32_t kDescO = tc::instruction(128, 256, true);
+            const uint32_t desc_q = tc::operand(base + kSmemQ, 0);
+            const uint32_t desc_a = tc::operand(base + kSmemA, 0);
+            const uint32_t desc_b = tc::operand(base + kSmemB, 0);
+            const uint32_t desc_v = tc::operand(base + kSmemB, kBlock);
+            auto wait = [&](uint32_t b, uint32_t parity) { return tc::mbar_wait(b, parity & 1, dead); };
+            // four blocks of latents with q's 0..255 (shared memory) or 256..511 (tensor memory)
+            auto low = [&](uint32_t rows) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    tc::mma_ss(kColS, desc_q + i * (kQBlock / 16) + 2 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
-        };
-        auto high = [&](uint32_t rows) {
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma_ss(kColS, desc_q + i * (kQBlock / 16) + 2 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+            };
+            auto high = [&](uint32_t rows) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    tc::mma_ts(kColS, kColQ + i * 32 + 8 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
-        };
-        auto rope = [&] {  // the first product of a tile's scores
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                tc::mma_ts(kColS, kColQ + 4 * 32 + 8 * k, desc_a + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
-        };
-        auto scores = [&](uint32_t n, int half) {
-            if (n >= 1 && !warp_wait(bar(kScoresRead), n - 1)) return false;
-            if (!warp_wait(bar(kFullA), n)) return false;
-            tc::fence_after();
-            if (tc::elect_one()) {
-                rope();
-                if (half) low(desc_a);
-                else high(desc_a);
-                tc::commit(bar(kFreeA));
-            }
-            __syncwarp();
-            if (!warp_wait(bar2(kFullB, n), n >> 1)) return false;
-            tc::fence_after();
-            if (tc::elect_one()) {
-                const uint32_t rows = desc_b + (n & 1) * (4 * kBlock / 16);
-                if (half) high(rows);
-                else low(rows);
-                tc::commit(bar(kScores));
-            }
-            __syncwarp();
-            return true;
-        };
-        auto output = [&](uint32_t n, bool accumulate) {
-            if (!warp_wait(bar(kWeights), n)) return false;
-            tc::fence_after();
-            if (tc::elect_one()) {
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma_ts(kColS, kColQ + i * 32 + 8 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+            };
+            auto output = [&](uint32_t n, bool accumulate) {
+                if (!wait(bar(kWeights), n)) return false;
+                tc::fence_after();
                 const uint32_t v = desc_v + (n & 1) * (4 * kBlock / 16);
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
                     tc::mma_ts(kColO, kColP + 8 * k, v + k * (2048 / 16), kDescO, accumulate || k > 0);
                 tc::commit(bar2(kOutput, n));
+                return true;
+            };
+            uint32_t n = 0, segment = 0;
+            bool before_first = true;  // was tile n - 1 the first of its piece?
+            for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
+                const bool first = at.u == u0 || at.tile == 0;
+                const bool half = at.row >= op.tokens;
+                if (first) {
+                    // the token before is finished first: its weights do not depend on this one's q
+                    if (n > 0 && !output(n - 1, !before_first)) break;
+                    if (!wait(bar(kQuery), segment)) break;
+                    ++segment;
+                }
+                if (n >= 1 && !wait(bar(kScoresRead), n - 1)) break;
+                bool ok = true;
+#pragma unroll 1
+                for (int part = 0; ok && part < 2; ++part) {
+                    ok = part ? wait(bar2(kFullB, n), n >> 1) : wait(bar(kFullA), n);
+                    tc::fence_after();
+                    const uint32_t rows = part ? desc_b + (n & 1) * (4 * kBlock / 16) : desc_a;
+                    if (!part) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)  // rope; the tile's first product overwrites
+                            tc::mma_ts(kColS, kColQ + 4 * 32 + 8 * k, rows + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
+                    }
+                    if (half == (part == 0)) low(rows);
+                    else high(rows);
+                    tc::commit(part ? bar(kScores) : bar(kFreeA));
+                }
+                if (!ok) break;
+                if (!first && !output(n - 1, !before_first)) break;
+                before_first = first;
+                if (at.u + 1 == u1 && !output(n, !first)) break;
             }
-            __syncwarp();
-            return true;
-        };
-        uint32_t n = 0, segment = 0;
-        bool before_first = true;  // was tile n - 1 the first of its piece?
-        for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
-            const bool first = at.u == u0 || at.tile == 0;
-            if (first) {
-                // the token before is finished first: its weights do not depend on this one's q
-                if (n > 0 && !output(n - 1, !before_first)) break;
-                if (!warp_wait(bar(kQuery), segment)) break;
-                ++segment;
-            }
-            if (!scores(n, at.row >= op.tokens)) break;
-            if (!first && !output(n - 1, !before_first)) break;
-            before_first = first;
-            if (at.u + 1 == u1 && !output(n, !first)) break;
         }
+        __syncwarp();
     } else {
         // ---- softmax, a thread a head ----
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         const int head = tid;
-        // A token's q, zero for heads beyond the last: latents 0..255 to shared memory (asynchronous
-        // copies), the rest to tensor memory.  Every score of the token before must have been made.
+        auto softmax_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // these four warps
+        // A token's q, zero for heads beyond the last.  Its latents 256..511 pass through the shared blocks of
+        // 0..255 on their way to tensor memory, so that every load is of whole lines: with a thread a head
+        // they took 6 us a token.  Every score of the token before must have been made.
         auto load_q = [&](int32_t token) {
             const __nv_bfloat16* q = op.q + token * op.q_token;
-            const int c = tid & 7;
-#pragma unroll 1
-            for (int h = tid >> 3; h < 128; h += 16) {
-                const bool there = h < op.heads;
-                const __nv_bfloat16* from = q + (there ? h : 0) * op.q_head + c * 8;
-                const uint32_t to = base + kSmemQ + h * 128 + ((c ^ (h & 7)) << 4);
-                if (op.q_aligned) {
+            const bool mine_there = head < op.heads;
+            const __nv_bfloat16* mine = q + (mine_there ? head : 0) * op.q_head + kLatent;
+            uint4 rope[8];
+            if (op.q_aligned) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * kQBlock),
-                                     "l"(from + k * 64), "r"(there ? 16 : 0)
-                                     : "memory");
-                } else {
-                    for (int k = 0; k < 4; ++k) {
-                        const uint4 v = load_unaligned(from + k * 64, there);
-                        shared_store16(to + k * kQBlock, v.x, v.y, v.z, v.w);
+                for (int k = 0; k < 8; ++k) rope[k] = __ldg(reinterpret_cast<const uint4*>(mine) + k);
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < 8; ++k) {
+                    const uint4 v = load_unaligned(mine + k * 8);
+                    shared_store16(base + kSmemQ + head * 128 + k * 16, v.x, v.y, v.z, v.w);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) rope[k] = shared_load16(base + kSmemQ + head * 128 + k * 16);
+                softmax_sync();
+            }
+            const uint32_t to0 = base + kSmemQ + (tid >> 3) * 128 + (((tid ^ (tid >> 3)) & 7) << 4);
+#pragma unroll 1
+            for (int first = 256; first >= 0; first -= 256) {
+                const __nv_bfloat16* from = q + (tid >> 3) * op.q_head + first + (tid & 7) * 8;
+#pragma unroll 1
+                for (int h = tid >> 3, i = 0; i < 8; ++i, h += 16, from += 16 * op.q_head) {
+                    const bool there = h < op.heads;
+                    const __nv_bfloat16* src = there ? from : q;  // not read where not there
+                    const uint32_t to = to0 + i * 16 * 128;
+                    if (op.q_aligned || !there) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * kQBlock),
+                                         "l"(src + k * 64), "r"(there ? 16 : 0)
+                                         : "memory");
+                    } else {
+#pragma unroll 1
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 v = load_unaligned(from + k * 64);
+                            shared_store16(to + k * kQBlock, v.x, v.y, v.z, v.w);
+                        }
                     }
                 }
-            }
-            const bool there = head < op.heads;
-            const __nv_bfloat16* mine = q + (there ? head : 0) * op.q_head + 256;
-            uint4 w[2][8];  // one group of 64 values is on its way while the one before is stored
-            auto fetch = [&](int i, uint4 (&v)[8]) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                if (first == 0) break;
+                softmax_sync();
+#pragma unroll 1
+                for (int i = 0; i < 5; ++i) {
+                    uint32_t w[32];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const __nv_bfloat16* from = mine + i * 64 + k * 8;
-                    v[k] = op.q_aligned ? __ldg(reinterpret_cast<const uint4*>(from)) : load_unaligned(from, there);
+                    for (int k = 0; k < 8; ++k) {
+                        uint4 v = mine_there ? rope[k] : make_uint4(0, 0, 0, 0);
+                        if (i < 4) v = shared_load16(base + kSmemQ + i * kQBlock + head * 128 + ((k ^ (head & 7)) << 4));
+                        w[4 * k] = v.x;
+                        w[4 * k + 1] = v.y;
+                        w[4 * k + 2] = v.z;
+                        w[4 * k + 3] = v.w;
+                    }
+                    tc::tmem_store32(lanes + kColQ + i * 32, w);
                 }
-            };
-            fetch(0, w[0]);
-#pragma unroll
-            for (int i = 0; i < 5; ++i) {
-                if (i < 4) fetch(i + 1, w[(i + 1) & 1]);
-                uint32_t x[32];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[4 * k] = there ? w[i & 1][k].x : 0u;
-                    x[4 * k + 1] = there ? w[i & 1][k].y : 0u;
-                    x[4 * k + 2] = there ? w[i & 1][k].z : 0u;
-                    x[4 * k + 3] = there ? w[i & 1][k].w : 0u;
-                }
-                __syncwarp();
-                tc::tmem_store32(lanes + kColQ + i * 32, x);
+                softmax_sync();
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
             tc::fence_async_shared();
             tc::tmem_wait_store();
             tc::fence_before();
@@ -421,7 +410,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 m = -INFINITY;
                 l2 = 0;
                 // the next token's q to L2: its loads come between two tokens, where nothing hides them
-                const int64_t next = static_cast<int64_t>(at.row + 1) * tiles;
+                const int32_t next = (at.row + 1) * tiles;
                 if (next < u1 && head < op.heads) {
                     const __nv_bfloat16* q =
                         op.q + (at.row + 1 < op.tokens ? at.row + 1 : at.row + 1 - op.tokens) * op.q_token + head * op.q_head;
@@ -511,7 +500,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 l += odd;
                 if (!warp_wait(bar2(kOutput, n), n >> 1)) break;
                 tc::fence_after();
-                const int64_t row_start = static_cast<int64_t>(at.row) * tiles;
+                const int32_t row_start = at.row * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
                 if (whole) {
                     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -587,7 +576,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
     const int head = tid & 127, group = tid >> 7;
     const bool joins = blockIdx.y < 64;
     const int half = joins ? blockIdx.y >> 5 : 0;
-    const int64_t first = (half * static_cast<int64_t>(op.tokens) + token) * div.tiles;
+    const int32_t first = (half * op.tokens + static_cast<int32_t>(token)) * div.tiles;
     const int i0 = div.cta_of(first), i1 = div.cta_of(first + div.tiles - 1);
     if (joins && i0 == i1) return;  // written by its one CTA
     float m = -INFINITY, l = 0.0f;  // of the token's head, maximum in base 2
@@ -683,12 +672,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 Division wide_division(int64_t tokens, int64_t topk, int sms) {
-    Division d;
-    d.rows = static_cast<int32_t>(2 * tokens);
-    d.tiles = static_cast<int32_t>(topk > 0 ? (topk + kTile - 1) / kTile : 1);  // no entry: one empty tile
-    const int64_t units = d.units();
-    d.ctas = static_cast<int32_t>(units < sms ? units : sms);
-    return d;
+    return Division(2 * tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms);  // no entry: one empty tile
 }
 
 // Byte offsets of the scratch arrays; [4] is the size.

@@ -29,13 +29,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // every other wait of the block that polls the same flag gives up with it.
 constexpr int kSpinLimit = 1 << 18;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-    if (mbar_try(bar, parity)) return true;
-    for (int i = 0; i < kSpinLimit; ++i) {
-        if (mbar_try(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; !mbar_try(bar, parity); ++i) {
         if (*dead) return false;
+        if (i == kSpinLimit) *dead = 1;
     }
-    *dead = 1;
-    return false;
+    return true;
 }
 
 // One lane of a converged warp.
