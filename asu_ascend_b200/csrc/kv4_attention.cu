@@ -13,11 +13,11 @@ namespace {
 
 using namespace kv4;
 
-bool narrow(int64_t heads) {
-    static const int limit = getenv("KV4_LIMIT") ? atoi(getenv("KV4_LIMIT")) : 32;
-    return heads <= limit; }
+bool old() { static const bool o = getenv("KV4_OLD"); return o; }
+bool narrow(int64_t heads) { return heads <= 32; }
 
 int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+    if (!old()) return decode_workspace(tokens, heads, topk, weights);
     return narrow(heads) ? narrow_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
 }
 
@@ -71,5 +71,6 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     op.lse = lse;
     op.weights = topk ? static_cast<__nv_bfloat16*>(weights) : nullptr;
     op.status = status;
+    if (!old()) return launch_decode(s, op, workspace);
     return narrow(heads) ? launch_narrow(s, op, workspace) : launch_wide(s, op, workspace);
 }

@@ -7,8 +7,6 @@
 namespace asu {
 namespace kv4 {
 
-constexpr int kTile = 64;  // entries a tile
-
 struct Operands {
     const __nv_bfloat16* q;
     int64_t q_token, q_head;  // elements
@@ -81,6 +79,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return reinterpret_cast<const uint32_t&>(v);
 }
 
+// kv4_decode.cu
+int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
+int launch_decode(cudaStream_t stream, const Operands& op, void* workspace);
 // kv4_decode_narrow.cu: few heads, at a cost that grows with them in steps of 16 (up to 32) or 32.
 int64_t narrow_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
 int launch_narrow(cudaStream_t stream, const Operands& op, void* workspace);

@@ -4,16 +4,18 @@
 // tcgen05 kernel would be seven eighths padding.  m16n8k16 products take the heads as their 16 rows
 // (kMT such groups of 16 in a CTA) and the entries (scores) or latents (output) as their columns.
 //
-// A CTA of 8 warps takes tiles of 32 entries.  Warp w owns the latents 64 w .. 64 w + 63, for the scores and
-// for the output: it dequantises them once, into registers in the layout that the score products want
-// (entry g = lane / 4 of 8, values 16 c .. 16 c + 15 with c = lane % 4: one 8-byte load and one
-// scale), and turns the same registers into the output products' layout with movmatrix, a transposition
-// of 8 x 8 values.  No dequantised value goes through shared memory.  The price is that each warp's
-// scores are partial sums over its latents: they are added up through shared memory, by the threads
-// that then do the softmax (16 threads a row with one group of heads, 8 with two).
+// A CTA of 8 warps takes tiles of 32 entries: warp (d, e) has the latents 128 d .. 128 d + 127 of the entries
+// 16 e .. 16 e + 15, for the scores and for the output.  It dequantises them once, into registers in the
+// layout that the score products want (entry g = lane / 4 of 8, values 32 c .. 32 c + 31 with
+// c = lane % 4: one 16-byte load), and turns the same registers into the output products' layout with
+// movmatrix, a transposition of 8 x 8 values.  No dequantised value goes through shared memory.  The
+// price: a warp's scores are partial sums over its latents, added up through shared memory by the threads
+// that then do the softmax (16 threads a row with one group of heads, 8 with two); and its output is a
+// partial sum over its entries, added up once a token.  (Eight warps of 64 latents and all 32 entries
+// each took twice the instructions: 81 us instead of the time below.)
 //
-// Which 16 values of a latent row a product's k index means is free as long as both operands agree: k
-// index 2c, 2c + 1, 2c + 8, 2c + 9 of step s are the values 16 c + 4 s .. 16 c + 4 s + 3.
+// Which 4 values of a latent row a thread's k indexes mean is free as long as both operands agree: k index
+// 2c, 2c + 1, 2c + 8, 2c + 9 of step s are the values 32 c + 4 s .. 32 c + 4 s + 3.
 //
 // Rows come by asynchronous copies, kStages - 1 tiles ahead.  Two barriers a tile: partial scores
 // written, weights written.  One group of heads: 128 registers, two CTAs on an SM, whose phases fill each
@@ -26,18 +28,19 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kKeys = 32;  // entries a tile
-constexpr int kStages = 6;
-constexpr int kRawTile = kKeys * kRowBytes;
+constexpr int kStages = 5;
+constexpr int kRawRow = kRowBytes + 32;  // 16 words more than a multiple of 32: two rows' 64 bytes are all banks
 constexpr int kPartRow = kKeys + 8;      // floats; 8 more than a multiple of 32: no bank conflicts
 constexpr int kWeightRow = kKeys + 8;    // bf16
 constexpr float kMaxGrowth = 8.0f;       // the maximum moves when it grows by more than 2^8
 
 template <int kMT>
 struct Shared {
-    alignas(128) uint8_t raw[kStages][kRawTile];
-    float part[8][16 * kMT][kPartRow];       // each warp's partial scores
+    alignas(128) uint8_t raw[kStages][kKeys * kRawRow];
+    uint4 q[kMT][32][32];                    // q's latents by product operand: [step 8 d + s][lane]
+    uint4 rope[kMT][4][32];                  // and its rope part
+    float part[4][16 * kMT][kPartRow];       // each d's partial scores
     __nv_bfloat16 weights[16 * kMT][kWeightRow];
-    uint4 rope[kMT][4][32];                  // q's rope part by product operand: [step][lane]
     float row[16 * kMT];                     // a row's factor
     uint32_t there[kStages][8];              // four entries a warp: which are there
 };
@@ -66,20 +69,24 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-// 16 values of a head of q from any element on; zeros for a head that is not there.
-__device__ __forceinline__ void load_q16(const __nv_bfloat16* p, bool there, bool aligned, uint32_t (&w)[8]) {
+// kN pairs of values of a head of q, from any element on; zeros for a head that is not there.
+template <int kN>
+__device__ __forceinline__ void load_q(const __nv_bfloat16* p, bool there, bool aligned, uint32_t (&w)[kN]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 0;
+    for (int i = 0; i < kN; ++i) w[i] = 0;
     if (!there) return;
     if (aligned) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-        return;
-    }
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
+        for (int i = 0; i < kN; i += 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p) + i / 2);
+            w[i] = v.x, w[i + 1] = v.y;
+        }
+    } else {
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
+    }
 }
 
 template <int kMT>
@@ -92,6 +99,7 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
     constexpr int kMine = kKeys / kLanesRow;         // entries a thread: 2 or 4
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, c = lane & 3;
+    const int d = warp >> 1, e = warp & 1;
     const int srow = tid / kLanesRow, skey = (tid % kLanesRow) * kMine;
     const int u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
     const int padded = (op.heads + kRows - 1) / kRows * kRows;
@@ -100,41 +108,42 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
 
     // ---- copies: this warp's four rows of a tile, 26 lanes a row ----
     Walk ahead(div, u0);
-    auto slot_of = [&](const Walk& w) -> int32_t {
-        const int e = w.tile * kKeys + warp * 4 + lane;
-        if (lane >= 4 || w.u >= u1 || e >= op.topk) return kNotFound;
-        return __ldg(op.slots + (w.row % op.tokens) * op.slots_token + e);
+    int ahead_token = ahead.row % op.tokens;
+    auto slot_of_lane = [&]() -> int32_t {  // lane r < 4: the warp's row r of the tile ahead
+        const int entry = ahead.tile * kKeys + warp * 4 + lane;
+        if (lane >= 4 || ahead.u >= u1 || entry >= op.topk) return kNotFound;
+        return __ldg(op.slots + ahead_token * op.slots_token + entry);
     };
-    int32_t slot = slot_of(ahead);
+    int32_t slot = slot_of_lane();
+    const uint32_t copy_to = shared_address(sm.raw[0]) + warp * 4 * kRawRow + lane * 16;
     auto copy = [&](int stage) {
         if (ahead.u < u1) {
             const bool there = slot >= 0 && slot < op.pool_rows;
             if (!there && slot != kNotFound) bits |= ASU_ST_BAD_QUERY;
-            const uint32_t valid = __ballot_sync(0xffffffffu, there) & 15u;
+            const uint32_t valid = __ballot_sync(0xffffffffu, there);
             if (lane == 0) sm.there[stage][warp] = valid;
-            const uint64_t pool = reinterpret_cast<uint64_t>(op.pool) + static_cast<uint64_t>(ahead.row % op.tokens) * op.pool_token +
-                                  lane * 16;
-            const uint32_t to = shared_address(sm.raw[stage]) + warp * 4 * kRowBytes + lane * 16;
+            const int32_t read = there ? slot : 0;  // an entry that is not there: zeros, finite values of weight 0
+            const uint8_t* pool = op.pool + static_cast<uint64_t>(ahead_token) * op.pool_token + lane * 16;
+            const uint32_t to = copy_to + stage * (kKeys * kRawRow);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int32_t s = __shfl_sync(0xffffffffu, slot, r);
-                const bool t = (valid >> r) & 1u;  // an entry that is not there: zeros, finite values of weight 0
-                const uint64_t from = pool + static_cast<uint64_t>(t ? s : 0) * op.pool_pitch;
+                const uint8_t* from = pool + static_cast<uint64_t>(__shfl_sync(0xffffffffu, read, r)) * op.pool_pitch;
                 if (lane < kRowBytes / 16)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * kRowBytes), "l"(from),
-                                 "r"(t ? 16 : 0)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * kRawRow), "l"(from),
+                                 "r"((valid >> r) & 1u ? 16 : 0)
                                  : "memory");
             }
+            const int row = ahead.row;
             ahead.next(div);
-            slot = slot_of(ahead);
+            if (ahead.row != row && ++ahead_token == op.tokens) ahead_token = 0;
+            slot = slot_of_lane();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) copy(i);
 
-    uint32_t q[kMT][2][8];  // heads g and g + 8 of each group, this thread's 16 latents
-    float o[kMT][8][4];     // [8 pairs of latents] heads g, g + 8
+    float o[kMT][16][4];            // [pair of latents 32 c + 2 b][heads g, g + 8]
     float m = -INFINITY, l = 0.0f;  // of row srow; l: this thread's entries
     int stage = 0;
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -147,28 +156,28 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
         if (first) {
             const __nv_bfloat16* qt = op.q + token * op.q_token;
 #pragma unroll
-            for (int t = 0; t < kMT; ++t)
+            for (int t = 0; t < kMT; ++t) {
+                const int h0 = head0 + 16 * t + g, h1 = h0 + 8;
+                const __nv_bfloat16* q0 = qt + (h0 < op.heads ? h0 : 0) * op.q_head;
+                const __nv_bfloat16* q1 = qt + (h1 < op.heads ? h1 : 0) * op.q_head;
+                uint32_t a[8], b[8];
+                load_q(q0 + d * 128 + c * 32 + e * 16, h0 < op.heads, op.q_aligned, a);
+                load_q(q1 + d * 128 + c * 32 + e * 16, h1 < op.heads, op.q_aligned, b);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int h = head0 + 16 * t + 8 * i + g;
-                    load_q16(qt + (h < op.heads ? h : 0) * op.q_head + warp * 64 + c * 16, h < op.heads, op.q_aligned, q[t][i]);
+                for (int k = 0; k < 4; ++k)
+                    sm.q[t][8 * d + 4 * e + k][lane] = make_uint4(a[2 * k], b[2 * k], a[2 * k + 1], b[2 * k + 1]);
+                if (e == 0) {
+                    uint32_t x[2], y[2];
+                    load_q(q0 + kLatent + d * 16 + c * 4, h0 < op.heads, op.q_aligned, x);
+                    load_q(q1 + kLatent + d * 16 + c * 4, h1 < op.heads, op.q_aligned, y);
+                    sm.rope[t][d][lane] = make_uint4(x[0], y[0], x[1], y[1]);
                 }
-            if (warp < kMT) {  // the rope part, warp t for group t; read behind the barrier below
-                uint32_t r[2][8];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int h = head0 + 16 * warp + 8 * i + g;
-                    load_q16(qt + (h < op.heads ? h : 0) * op.q_head + kLatent + c * 16, h < op.heads, op.q_aligned, r[i]);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    sm.rope[warp][s][lane] = make_uint4(r[0][2 * s], r[1][2 * s], r[0][2 * s + 1], r[1][2 * s + 1]);
             }
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < kMT; ++t)
 #pragma unroll
-                for (int b = 0; b < 8; ++b)
+                for (int b = 0; b < 16; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[t][b][i] = 0.0f;
             m = -INFINITY;
@@ -176,48 +185,44 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
         }
 
         // ---- dequantise, partial scores ----
-        const uint8_t* raw = sm.raw[stage];
-        uint32_t v[4][8];  // [8 entries][pairs of latents]
-        float s[kMT][4][4];
+        const uint8_t* raw = sm.raw[stage] + (16 * e + g) * kRawRow;
+        uint32_t v[2][16];  // [8 entries][pairs of latents]
+        float s[kMT][2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint8_t* row = raw + (8 * j + g) * kRowBytes;
-            const uint2 code = *reinterpret_cast<const uint2*>(row + warp * 32 + c * 8);
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t* row = raw + 8 * j * kRawRow;
+            const uint4 code = *reinterpret_cast<const uint4*>(row + d * 64 + c * 16);
+            const uint32_t scales = *reinterpret_cast<const unsigned short*>(row + kScaleOffset + d * 8 + c * 2);
+            const uint2 rope = *reinterpret_cast<const uint2*>(row + kRopeOffset + d * 32 + c * 8);
             __nv_bfloat162 sc, cc;
-            scale_pair(row[kScaleOffset + warp * 4 + c], sc, cc);
+            scale_pair(scales, 0, sc, cc);
             unpack_word(code.x, sc, cc, &v[j][0]);
             unpack_word(code.y, sc, cc, &v[j][4]);
+            scale_pair(scales, 1, sc, cc);
+            unpack_word(code.z, sc, cc, &v[j][8]);
+            unpack_word(code.w, sc, cc, &v[j][12]);
 #pragma unroll
             for (int t = 0; t < kMT; ++t) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[t][j][i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma(s[t][j], make_uint4(q[t][0][2 * k], q[t][1][2 * k], q[t][0][2 * k + 1], q[t][1][2 * k + 1]),
-                        v[j][2 * k], v[j][2 * k + 1]);
+                mma(s[t][j], sm.rope[t][d][lane], rope.x, rope.y);
             }
         }
-        {  // rope: warp w takes the entries 8 (w % 4) .. and two of the four steps
-            const int j = warp & 3, k0 = (warp >> 2) * 2;
-            const uint4 r = *reinterpret_cast<const uint4*>(raw + (8 * j + g) * kRowBytes + kRopeOffset + c * 32 + k0 * 8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int t = 0; t < kMT; ++t) {
-                float x[4] = {};
-                mma(x, sm.rope[t][k0][lane], r.x, r.y);
-                mma(x, sm.rope[t][k0 + 1][lane], r.z, r.w);
+                const uint4 a = sm.q[t][8 * d + k][lane];
 #pragma unroll
-                for (int jj = 0; jj < 4; ++jj)
-                    if (jj == j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[t][jj][i] += x[i];
+                for (int j = 0; j < 2; ++j) mma(s[t][j], a, v[j][2 * k], v[j][2 * k + 1]);
             }
-        }
 #pragma unroll
         for (int t = 0; t < kMT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                *reinterpret_cast<float2*>(&sm.part[warp][16 * t + g][8 * j + 2 * c]) = make_float2(s[t][j][0], s[t][j][1]);
-                *reinterpret_cast<float2*>(&sm.part[warp][16 * t + g + 8][8 * j + 2 * c]) = make_float2(s[t][j][2], s[t][j][3]);
+            for (int j = 0; j < 2; ++j) {
+                float* to = &sm.part[d][16 * t + g][16 * e + 8 * j + 2 * c];
+                *reinterpret_cast<float2*>(to) = make_float2(s[t][j][0], s[t][j][1]);
+                *reinterpret_cast<float2*>(to + 8 * kPartRow) = make_float2(s[t][j][2], s[t][j][3]);
             }
         __syncthreads();
         copy(stage == 0 ? kStages - 1 : stage - 1);  // the tile before has been read
@@ -225,16 +230,15 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
         // ---- softmax: kLanesRow threads a row ----
         float x[kMine];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) x[i] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const float* from = &sm.part[w][srow][skey];
             if constexpr (kMine == 2) {
                 const float2 y = *reinterpret_cast<const float2*>(from);
-                x[0] += y.x, x[1] += y.y;
+                x[0] = w ? x[0] + y.x : y.x, x[1] = w ? x[1] + y.y : y.y;
             } else {
                 const float4 y = *reinterpret_cast<const float4*>(from);
-                x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+                x[0] = w ? x[0] + y.x : y.x, x[1] = w ? x[1] + y.y : y.y;
+                x[2] = w ? x[2] + y.z : y.z, x[3] = w ? x[3] + y.w : y.w;
             }
         }
         const uint32_t there = sm.there[stage][skey >> 2] >> (skey & 3);
@@ -245,7 +249,7 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
             top = fmaxf(top, x[i]);
         }
 #pragma unroll
-        for (int d = kLanesRow / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int k = kLanesRow / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         float fade = 1.0f;
         if (first) {
             m = top;
@@ -278,72 +282,91 @@ kv4_decode_narrow_kernel(const Operands op, const Division div, const NarrowScra
             for (int t = 0; t < kMT; ++t) {
                 const float f0 = sm.row[16 * t + g], f1 = sm.row[16 * t + g + 8];
 #pragma unroll
-                for (int b = 0; b < 8; ++b) o[t][b][0] *= f0, o[t][b][1] *= f0, o[t][b][2] *= f1, o[t][b][3] *= f1;
+                for (int b = 0; b < 16; ++b) o[t][b][0] *= f0, o[t][b][1] *= f0, o[t][b][2] *= f1, o[t][b][3] *= f1;
             }
         }
 
         // ---- output ----
+        uint4 a[kMT];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint4 a[kMT];
+        for (int t = 0; t < kMT; ++t)
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(a[t].x), "=r"(a[t].y), "=r"(a[t].z), "=r"(a[t].w)
+                         : "r"(shared_address(&sm.weights[16 * t + (lane & 15)][16 * e + (lane >> 4) * 8])));
 #pragma unroll
-            for (int t = 0; t < kMT; ++t)
-                asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(a[t].x), "=r"(a[t].y), "=r"(a[t].z), "=r"(a[t].w)
-                             : "r"(shared_address(&sm.weights[16 * t + (lane & 15)][16 * k + (lane >> 4) * 8])));
+        for (int b = 0; b < 16; ++b) {
+            const uint32_t b0 = transpose8x8(v[0][b]), b1 = transpose8x8(v[1][b]);
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                const uint32_t b0 = transpose8x8(v[2 * k][b]), b1 = transpose8x8(v[2 * k + 1][b]);
-#pragma unroll
-                for (int t = 0; t < kMT; ++t) mma(o[t][b], a[t], b0, b1);
-            }
+            for (int t = 0; t < kMT; ++t) mma(o[t][b], a[t], b0, b1);
         }
 
         if (last) {
+            // the two halves of the entries, 64 latents at a time, through q's place
+            float4* half = reinterpret_cast<float4*>(sm.q);
 #pragma unroll
-            for (int d = kLanesRow / 2; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+            for (int t = 0; t < kMT; ++t)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    __syncthreads();  // q, or the round before, has been read
+                    if (e == 1)
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            const float* x = o[t][8 * r + b];
+                            half[(d * 8 + b) * 32 + lane] = make_float4(x[0], x[1], x[2], x[3]);
+                        }
+                    __syncthreads();
+                    if (e == 0)
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            const float4 x = half[(d * 8 + b) * 32 + lane];
+                            float* y = o[t][8 * r + b];
+                            y[0] += x.x, y[1] += x.y, y[2] += x.z, y[3] += x.w;
+                        }
+                }
+#pragma unroll
+            for (int k = kLanesRow / 2; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
             const int row_start = at.row * div.tiles;
             const bool whole = row_start >= u0 && row_start + div.tiles <= u1;
-            __syncthreads();  // sm.row has been read
-            if (whole) {
-                if (tid % kLanesRow == 0) {
+            const int piece = div.piece(blockIdx.x, row_start);
+            if (tid % kLanesRow == 0) {
+                if (whole) {
                     sm.row[srow] = l > 0.0f ? 1.0f / l : 0.0f;
                     if (head0 + srow < op.heads)
                         op.lse[static_cast<int64_t>(token) * op.heads + head0 + srow] =
                             l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-                }
-                __syncthreads();
-#pragma unroll
-                for (int t = 0; t < kMT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int h = head0 + 16 * t + 8 * i + g;
-                        if (h >= op.heads) continue;
-                        const float f = sm.row[16 * t + 8 * i + g];
-                        uint32_t w[8];
-#pragma unroll
-                        for (int b = 0; b < 8; ++b) w[b] = pack_bf16(o[t][b][2 * i] * f, o[t][b][2 * i + 1] * f);
-                        uint4* to = reinterpret_cast<uint4*>(op.out + (static_cast<int64_t>(token) * op.heads + h) * kLatent +
-                                                             warp * 64 + c * 16);
-                        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                        to[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
-            } else {
-                const int piece = div.piece(blockIdx.x, row_start);
-                if (tid % kLanesRow == 0) {
+                } else {
                     scratch.ml[piece * 2 * kRows + srow] = m;
                     scratch.ml[(piece * 2 + 1) * kRows + srow] = l;
                 }
+            }
+            __syncthreads();
+            if (e == 0) {
 #pragma unroll
                 for (int t = 0; t < kMT; ++t)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float4* to = reinterpret_cast<float4*>(
-                            scratch.o + (static_cast<int64_t>(piece) * kRows + 16 * t + 8 * i + g) * kLatent + warp * 64 + c * 16);
+                        const int r = 16 * t + 8 * i + g, h = head0 + r;
+                        if (whole) {
+                            if (h >= op.heads) continue;
+                            const float f = sm.row[r];
+                            uint4* to = reinterpret_cast<uint4*>(
+                                op.out + (static_cast<int64_t>(token) * op.heads + h) * kLatent + d * 128 + c * 32);
 #pragma unroll
-                        for (int b = 0; b < 4; ++b)
-                            to[b] = make_float4(o[t][2 * b][2 * i], o[t][2 * b][2 * i + 1], o[t][2 * b + 1][2 * i],
-                                                o[t][2 * b + 1][2 * i + 1]);
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int b = 0; b < 4; ++b)
+                                    w[b] = pack_bf16(o[t][4 * k + b][2 * i] * f, o[t][4 * k + b][2 * i + 1] * f);
+                                to[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+                            float4* to = reinterpret_cast<float4*>(
+                                scratch.o + (static_cast<int64_t>(piece) * kRows + r) * kLatent + d * 128 + c * 32);
+#pragma unroll
+                            for (int b = 0; b < 8; ++b)
+                                to[b] = make_float4(o[t][2 * b][2 * i], o[t][2 * b][2 * i + 1], o[t][2 * b + 1][2 * i],
+                                                    o[t][2 * b + 1][2 * i + 1]);
+                        }
                     }
             }
         }

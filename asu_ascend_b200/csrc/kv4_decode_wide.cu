@@ -27,6 +27,7 @@ namespace {
 //
 // The running maximum only moves when it grows by more than 2^8: until then the weights stay below
 // 2^8, as exact in bf16 as any others, and the output needs no rescaling.
+constexpr int kTile = 64;  // entries a tile
 constexpr int kWideThreads = 15 * 32;
 constexpr int kBlock = kTile * 128;  // bytes of a [64 x 64] bf16 block
 constexpr int kQBlock = 128 * 128;   // bytes of a [128 x 64] bf16 block
@@ -257,8 +258,8 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         // ---- the products, all by one lane.  (The branch has to be that of elect.sync itself: with a plain
         // lane number, or its result kept, the issue of a product takes 80 cycles instead of 30.) ----
         if (tc::elect_one()) {
-            constexpr uint32_t kDescS = tc::instruction(128, kTile, false);
-            constexpr uint32_t kDescO = tc::instruction(128, 256, true);
+            constexpr uint32_t kDescS = tc::instruction(128, kTile, false, false);
+            constexpr uint32_t kDescO = tc::instruction(128, 256, false, true);
             const uint32_t desc_q = tc::operand(base + kSmemQ, 0);
             const uint32_t desc_a = tc::operand(base + kSmemA, 0);
             const uint32_t desc_b = tc::operand(base + kSmemB, 0);
@@ -387,7 +388,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                         w[4 * k + 2] = v.z;
                         w[4 * k + 3] = v.w;
                     }
-                    tc::tmem_store32(lanes + kColQ + i * 32, w);
+                    tc::tmem_store(lanes + kColQ + i * 32, w);
                 }
                 softmax_sync();
             }
@@ -429,8 +430,8 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             if (!warp_wait(bar(kScores), n)) break;
             tc::fence_after();
             uint32_t s[2][32];
-            tc::tmem_load32(lanes + kColS, s[0]);
-            tc::tmem_load32(lanes + kColS + 32, s[1]);
+            tc::tmem_load(lanes + kColS, s[0]);
+            tc::tmem_load(lanes + kColS + 32, s[1]);
             tc::tmem_wait_load(s[0]);
             tc::tmem_wait_load(s[1]);
             tc::fence_before();
@@ -462,11 +463,11 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
 #pragma unroll 1
                 for (int c = 0; c < 256; c += 32) {
                     uint32_t o[32];
-                    tc::tmem_load32(lanes + kColO + c, o);
+                    tc::tmem_load(lanes + kColO + c, o);
                     tc::tmem_wait_load(o);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fade);
-                    tc::tmem_store32(lanes + kColO + c, o);
+                    tc::tmem_store(lanes + kColO + c, o);
                 }
             }
             const uint64_t scale2 = pair(__float_as_uint(op.scale_log2), __float_as_uint(op.scale_log2));
@@ -481,7 +482,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 l2 = add2(l2, pair(__float_as_uint(a), __float_as_uint(b)));
                 p[i] = pack_bf16(a, b);
             }
-            tc::tmem_store32(lanes + kColP, p);
+            tc::tmem_store(lanes + kColP, p);
             tc::tmem_wait_store();
             tc::fence_before();
             tc::mbar_arrive(bar(kWeights));
@@ -508,7 +509,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
 #pragma unroll 1
                     for (int c = 0; c < 256; c += 32) {
                         uint32_t o[32];
-                        tc::tmem_load32(lanes + kColO + c, o);
+                        tc::tmem_load(lanes + kColO + c, o);
                         tc::tmem_wait_load(o);
                         if (head < op.heads) {
 #pragma unroll
@@ -532,7 +533,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
 #pragma unroll 1
                     for (int c = 0; c < 256; c += 32) {
                         uint32_t o[32];
-                        tc::tmem_load32(lanes + kColO + c, o);
+                        tc::tmem_load(lanes + kColO + c, o);
                         tc::tmem_wait_load(o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) to[(c + i) * 128] = __uint_as_float(o[i]);
