@@ -4,33 +4,16 @@
 //   out_h = sum_j p_hj v_j,  p_h = softmax(s_h),  v_j = the first 512 of k_j
 //   lse_h = log sum_j exp s_hj,   weights_j = sum_h p_hj
 // A token without any entry: out 0, lse -inf, weights 0.
-#include <cstdlib>
-
 #include "kv4_decode.cuh"
 
-namespace asu {
-namespace {
-
-using namespace kv4;
-
-bool old() { static const bool o = getenv("KV4_OLD"); return o; }
-bool narrow(int64_t heads) { return heads <= 32; }
-
-int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
-    if (!old()) return decode_workspace(tokens, heads, topk, weights);
-    return narrow(heads) ? narrow_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
-}
-
-}  // namespace
-}  // namespace asu
-
 using namespace asu;
+using namespace asu::kv4;
 
 extern "C" int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights) {
     if (tokens < 0 || heads < 0 || topk < 0 || tokens > ASU_KV4_MAX_TOKENS || heads > ASU_KV4_MAX_HEADS ||
         topk > ASU_KV4_MAX_TOPK)
         return -1;
-    return workspace_bytes(tokens, heads, topk, weights != 0);
+    return tokens && heads ? decode_workspace(tokens, heads, topk, weights != 0) : 0;
 }
 
 extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -45,7 +28,7 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
         return ASU_ERR_ARG;
     if (tokens == 0 || heads == 0) return ASU_OK;
     if (!q || !out || !lse || (topk && (!slots || !pool))) return ASU_ERR_ARG;
-    const int64_t need = workspace_bytes(tokens, heads, topk, weights != nullptr);
+    const int64_t need = decode_workspace(tokens, heads, topk, weights != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_size < need)) return ASU_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(pool) % 16 || pool_pitch % 16 ||
         pool_token_stride % 16 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(lse) % 4 ||
@@ -71,6 +54,5 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     op.lse = lse;
     op.weights = topk ? static_cast<__nv_bfloat16*>(weights) : nullptr;
     op.status = status;
-    if (!old()) return launch_decode(s, op, workspace);
-    return narrow(heads) ? launch_narrow(s, op, workspace) : launch_wide(s, op, workspace);
+    return launch_decode(s, op, workspace);
 }

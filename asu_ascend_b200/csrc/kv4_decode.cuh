@@ -82,12 +82,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // kv4_decode.cu
 int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
 int launch_decode(cudaStream_t stream, const Operands& op, void* workspace);
-// kv4_decode_narrow.cu: few heads, at a cost that grows with them in steps of 16 (up to 32) or 32.
-int64_t narrow_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
-int launch_narrow(cudaStream_t stream, const Operands& op, void* workspace);
-// kv4_decode_wide.cu: any number of heads up to 128, at the cost of 128.
-int64_t wide_workspace(int64_t tokens, int64_t topk, bool weights);
-int launch_wide(cudaStream_t stream, const Operands& op, void* workspace);
 
 }  // namespace kv4
 }  // namespace asu

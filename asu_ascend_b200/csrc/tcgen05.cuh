@@ -44,12 +44,13 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
-// Whether any of the first 128 threads says so; all of them meet here.
-__device__ __forceinline__ bool any_of_128(bool here) {
+// Whether any of the first kCount threads says so; all of them meet here, at named barrier 1.
+template <int kCount>
+__device__ __forceinline__ bool any_of(bool here) {
     uint32_t r;
-    asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
+    asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, %2, p; selp.u32 %0, 1, 0, q; }"
                  : "=r"(r)
-                 : "r"(static_cast<uint32_t>(here))
+                 : "r"(static_cast<uint32_t>(here)), "n"(kCount)
                  : "memory");
     return r != 0;
 }
@@ -71,7 +72,17 @@ __device__ __forceinline__ void tmem_free(uint32_t base) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(kColumns) : "memory");
 }
 
-// 16 or 32 columns of the warp's 32 lanes: a thread holds one lane.
+// 4, 8, 16 or 32 columns of the warp's 32 lanes: a thread holds one lane.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -112,22 +123,31 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[4]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) : : "memory");
+}
 __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand in 128-byte swizzled atoms (8 rows of 128 bytes, 1024-byte aligned).
-//   K-major (rows are M or N, 64 elements of K a row): `stride` between 8-row groups, `lead` unused.
-//   MN-major (rows are K, 64 elements of M or N a row): `lead` between 64-element blocks of M or N,
-//   `stride` between groups of 8 K.
+// Shared-memory operand in swizzled groups of 8 rows, 1024-byte aligned.
+//   K-major: rows are M or N, and hold K; `lead` unused.
+//   MN-major: rows are K, and hold M or N; `lead` between blocks of a row's width of M or N.
 // Its descriptor's lower half holds the address (units of 16 bytes; advancing within the operand is an
 // addition), the upper half depends on the layout alone and is an immediate of the products below: with
 // both halves in ordinary registers the moves to uniform ones took longer than the products.
 __device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
     return ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);
 }
-constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024
+// Rows of 128 bytes in the 128-byte swizzle (16-byte chunk ^ row % 8), or of 64 bytes in the 64-byte one
+// (chunk ^ row / 2 % 4); 8-row groups follow one another.
+__host__ __device__ constexpr uint32_t operand_high(int row_bytes) {
+    return (static_cast<uint32_t>(row_bytes) * 8 >> 4) | (1u << 14) | ((row_bytes == 128 ? 2u : 4u) << 29);
+}
 
 // kind::f16: bf16 x bf16 -> fp32, M x N, K = 16.
 __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_m_major, bool b_n_major) {
@@ -135,21 +155,13 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_m_major,
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+template <uint32_t kHighA, uint32_t kHighB>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{ .reg .pred p; .reg .b64 x, y; setp.ne.u32 p, %4, 0;\n"
-        "mov.b64 x, {%1, %5}; mov.b64 y, {%2, %5};\n"
+        "mov.b64 x, {%1, %5}; mov.b64 y, {%2, %6};\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh)
-        : "memory");
-}
-// A from tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; .reg .b64 y; setp.ne.u32 p, %4, 0;\n"
-        "mov.b64 y, {%2, %5};\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh)
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHighA), "n"(kHighB)
         : "memory");
 }
 // The barrier completes when every tcgen05.mma issued by this thread so far has.
