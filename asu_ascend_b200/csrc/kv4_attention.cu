@@ -9,6 +9,16 @@
 using namespace asu;
 using namespace asu::kv4;
 
+// Up to kTallHeads heads the kernel whose products have the heads as columns, above it the one whose products
+// have them as 128 rows.  One and the other in us, 2048 entries:
+//   heads            16        32        64        80       128
+//   128 tokens  52 / 115  64 / 116  95 / 118  167 / 120  181 / 125
+//   32 tokens   22 /  57  26 /  57  35 /  58   54 /  58   56 /  59
+//   1 token     17 /  17  17 /  17  18 /  16   19 /  16   18 /  16
+static int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+    return heads <= kTallHeads ? tall_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
+}
+
 extern "C" int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights) {
     if (tokens < 0 || heads < 0 || topk < 0 || tokens > ASU_KV4_MAX_TOKENS || heads > ASU_KV4_MAX_HEADS ||
         topk > ASU_KV4_MAX_TOPK)
@@ -54,5 +64,5 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     op.lse = lse;
     op.weights = topk ? static_cast<__nv_bfloat16*>(weights) : nullptr;
     op.status = status;
-    return launch_decode(s, op, workspace);
+    return op.heads <= kTallHeads ? launch_tall(s, op, workspace) : launch_wide(s, op, workspace);
 }

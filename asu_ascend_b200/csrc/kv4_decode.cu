@@ -1,32 +1,36 @@
-// Sparse decode attention over the 4-bit cache, on the tcgen05 tensor cores.
+// Sparse decode attention over the 4-bit cache for up to 64 heads, on the tcgen05 tensor cores.
 //
 // A row of 416 bytes meets 1088 multiply-adds for each head.  The products take the 128 entries of a tile
 // (scores) or 128 latents (output) as their 128 rows and the heads as their columns, so that few heads
 // cost little more than the reading of the dequantised rows from shared memory:
 //   scores  S^T [128 entries x kN heads] = K Q^T          36 products of K = 16
 //   output  O^T [4 x 128 latents x kN]  += V^T P^T        32 products
-// Heads are taken kN = 16 or 32 at a time; more are several rows of work.
+// Heads are padded to kN = 16, 32 or 64 (a product with both operands in shared memory takes 40 cycles for
+// 32 columns or fewer, 48 for 64).
 //
-// Shared memory, 225 KB with 32 heads: q, 9 blocks of [kN heads x 64 values]; the tile's dequantised rows, 8
+// Shared memory, 217 KB with 64 heads: q, 9 blocks of [kN heads x 64 values]; the tile's dequantised rows, 8
 // blocks of [128 entries x 64 latents] and one of the rope part, all 128-byte rows in the 128-byte
-// swizzle; the weights P [128 entries x kN]; and the 4-bit part of the next tile's rows.  A latent block
-// serves both products: entries x latents with the latents contiguous is K-major for the scores and M-major
-// for the output.  There is no room for a second dequantised tile; its parts are released one after the
-// other instead: the rope block after the scores, latents 0..255 after the first half of the output
-// products, the rest after the second, and the scores' products start on a part while the next is filled.
+// swizzle.  A latent block serves both products: entries x latents with the latents contiguous is K-major
+// for the scores and M-major for the output.  The weights P [128 entries x kN] take the rope block's
+// place once the scores are made.  There is no room for a second tile; its parts are released one after the
+// other instead: latents 0..255 after the first half of the output products, the rest after the second,
+// and the scores' products start on a part while the next is being filled.
 //
-// Tensor memory: O^T 4 kN columns, S^T kN.  A thread's lane is an entry, so the maximum over the entries would
-// be an exchange between 128 threads.  It is not needed in every tile: any reference close to it will do, as
-// bf16 and fp32 carry 2^-126 .. 2^127.  The reference is the maximum of a piece's first tile and moves
-// only when a score exceeds it by 2^40, which the threads vote on.  Sums of the weights stay with the
-// threads until the piece is done.
+// Tensor memory: O^T 4 kN columns, S^T kN.  A softmax thread's lane is an entry, so it holds all the heads of
+// its entry and the maximum over the entries would be an exchange between 128 threads.  It is not needed in
+// every tile: any reference close to it will do, as bf16 and fp32 carry 2^-126 .. 2^127.  The
+// reference is the maximum of a piece's first tile and moves only when a score exceeds it by 2^40,
+// which the threads vote on.  Sums of the weights stay with the threads until the piece is done.
 //
-// 19 warps.  Dequantising a tile, its scores, their softmax and the output products wait for one another
-// all around, so the same 16 warps do both kinds of work, each kind in a quarter of the time that four
-// warps of its own took: they dequantise the tile, and when the scores are there, four warps a quarter of
-// the entries make a quarter of the heads each.  Two warps copy rows, asynchronously (a tile's 53 KB on
-// their way to registers instead do not fit into what the shared memory leaves of the L1 cache: their issue
-// alone took 2 us).  One issues the products.
+// 13 warps: 4 softmax, 8 that load rows into registers and dequantise (the next tile's loads are issued as
+// soon as a tile is stored, and fly during its products), one that issues the products.
+//
+// 128 tokens x 16 heads x 2048 entries take 56 us, 61 x 64 x 1024 35 us.  A tile is a chain of 3.4 us: the
+// output products of its first half 0.35, two halves to dequantise 0.7 to 0.85 each (shared-memory stores: 128
+// KB are 1000 cycles), the scores' second half 0.45, the softmax 0.45, four hand-overs of 0.15; the loads of
+// rows are hidden.  Tried and slower: tiles of 64 entries twice (both buffers are held while one is filled:
+// 78 us), rows through asynchronous copies and 16 warps that dequantise and make the softmax (62 us), products
+// of single warps with rows dequantised in registers (79 us).
 #include "kv4_decode.cuh"
 #include "tcgen05.cuh"
 
@@ -34,27 +38,21 @@ namespace asu {
 namespace kv4 {
 namespace {
 
-constexpr int kWorkers = 16 * 32;
-constexpr int kThreads = kWorkers + 3 * 32;
+constexpr int kThreads = 13 * 32;
 constexpr int kTile = 128;
-constexpr int kBlock = kTile * 128;        // bytes of a [128 entries x 64] block
-constexpr int kRawHalf = kTile * (128 + 16);  // bytes of a tile's 256 latents in 4 bits: nibbles, then scales
+constexpr int kBlock = kTile * 128;  // bytes of a [128 entries x 64] block
 constexpr float kMaxGrowth = 40.0f;  // base 2
 
 // Every barrier is waited for in every phase by each of its waiters, and its next phase depends on them: a
 // phase is never two ahead of one that waits for it.
 enum Bar {
-    kLowHere,   // the 4-bit latents 0..255 of the tile are in shared memory (64 threads' copies)
-    kLowRead,   // and have been read (16 warps)
-    kHighHere,  // the same of 256..511
-    kHighRead,
-    kFullLow,   // latents 0..255 of the tile are dequantised (16 warps)
-    kFullHigh,  // 256..511 (16 warps) and the rope part (2)
+    kFullLow,   // latents 0..255 of the tile are dequantised (8 warps)
+    kFullHigh,  // 256..511 and rope (8 warps)
     kFreeLow,   // the output products of latents 0..255 are done
     kOutput,    // all of them: the rest of the rows and the weights are free
     kScores,    // the tile's scores are made
-    kWeights,   // its weights are in shared memory and the scores read (16 warps)
-    kQuery,     // the row of work's q is in place (16 warps)
+    kWeights,   // its weights are in shared memory and the scores read (128 threads)
+    kQuery,     // the row of work's q is in place (128 threads)
     kDrain,
     kBars
 };
@@ -62,16 +60,12 @@ enum Bar {
 template <int kN>
 struct Layout {
     static constexpr int kQBlock = kN * 128;  // bytes of a [kN heads x 64] block
-    static constexpr int kWeightRow = kN == 32 ? 64 : 128;  // bytes; with 16 heads there is room for padding
     static constexpr int kQ = 0;
-    static constexpr int kRows = 9 * kQBlock;
-    static constexpr int kRope = kRows + 8 * kBlock;
-    static constexpr int kP = kRope + kBlock;
-    static constexpr int kRaw = kP + kTile * kWeightRow;
-    static constexpr int kBarsAt = kRaw + 2 * kRawHalf;
+    static constexpr int kRows = (9 * kQBlock + 1023) / 1024 * 1024;
+    static constexpr int kRope = kRows + 8 * kBlock;  // later the weights
+    static constexpr int kBarsAt = kRope + kBlock;
     static constexpr int kBytes = kBarsAt + 8 * kBars + 1024;  // the base is rounded up to 1024
     static constexpr uint32_t kColS = 4 * kN;
-    static_assert(kRows % 1024 == 0 && kP % 1024 == 0, "swizzled blocks start on 1024 bytes");
 };
 
 struct Scratch {
@@ -81,45 +75,28 @@ struct Scratch {
     __nv_bfloat16* p;  // [rows of work][tiles][128][kN] a tile's weights
 };
 
-__device__ __forceinline__ void shared_store16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
+// What a slot that is not there reads: a row of zeros.
+__device__ __align__(16) const uint32_t g_zero_row[kRowBytes / 4] = {
+#define ASU_ZERO4 0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u
+#define ASU_ZERO16 ASU_ZERO4, ASU_ZERO4, ASU_ZERO4, ASU_ZERO4
+    ASU_ZERO16, ASU_ZERO16, ASU_ZERO16, ASU_ZERO16
+#undef ASU_ZERO16
+#undef ASU_ZERO4
+};
 
-__device__ __forceinline__ uint4 shared_load16(uint32_t at) {
+// Loads that stay where they are written: the compiler would move plain ones down to their use and expose
+// their latency.
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
     uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
     return v;
 }
-__device__ __forceinline__ uint32_t shared_load2(uint32_t at) {
+__device__ __forceinline__ uint32_t load2(const uint8_t* p) {
     unsigned short v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
     return v;
-}
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {  // zeros where not there
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-
-// 32 latents as four 16-byte chunks of a swizzled row; chunk i goes to `at` with i in address bits 4 and 5.
-__device__ __forceinline__ void dequantise(const uint4& code, uint32_t scales, uint32_t at) {
-    const uint32_t w[4] = {code.x, code.y, code.z, code.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __nv_bfloat162 s, c;
-        scale_pair(scales, i / 2, s, c);
-        uint32_t v[4];
-        unpack_word(w[i], s, c, v);
-        shared_store16(at ^ (i << 4), v[0], v[1], v[2], v[3]);
-    }
-}
-
-// 8 values that start on any element.
-__device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
-    uint32_t w[4];
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Floats in the order of signed integers, and back.
@@ -129,35 +106,6 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 
-template <int kC>
-__device__ __forceinline__ void load_shared(float (&v)[kC], const float* from) {
-#pragma unroll
-    for (int i = 0; i < kC; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(from + i);
-        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
-    }
-}
-
-// The weights of an entry and 2 kW heads, the part-th such group, into the entry's row of chunks of 8 heads:
-// 128-byte rows, chunk ^ row % 8, or 64-byte rows, chunk ^ row / 2 % 4 ...
-template <int kW>
-__device__ __forceinline__ void store_weights(uint32_t base, int entry, int part, const uint32_t (&p)[kW]) {
-    if constexpr (kW == 2) {
-        const uint32_t to = base + entry * 128 + (((part >> 1) ^ (entry & 7)) << 4) + (part & 1) * 8;
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(p[0]), "r"(p[1]) : "memory");
-    } else {
-        shared_store16(base + entry * 64 + ((part ^ ((entry >> 1) & 3)) << 4), p[0], p[1], p[2], p[3]);
-    }
-}
-// ... and to global memory.
-template <int kW>
-__device__ __forceinline__ void store_weights(__nv_bfloat16* to, const uint32_t (&p)[kW]) {
-    if constexpr (kW == 2) *reinterpret_cast<uint2*>(to) = make_uint2(p[0], p[1]);
-    else *reinterpret_cast<uint4*>(to) = make_uint4(p[0], p[1], p[2], p[3]);
-}
-
-__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
-
 template <int kN>
 __global__ void __launch_bounds__(kThreads, 1)
 kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) {
@@ -165,9 +113,9 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
-    __shared__ __align__(16) float s_minus_ref[kN];  // minus the reference, base 2; +inf while there is none
-    __shared__ __align__(16) float s_fade[kN];       // what a new reference multiplies sums and output by; later 1 / sum
-    __shared__ int s_top[4][kN];                     // by quarters of the entries: maximum, or sum
+    __shared__ float s_minus_ref[kN];  // minus the reference, base 2; +inf while there is none
+    __shared__ float s_fade[kN];       // what a new reference multiplies sums and output by; later 1 / sum
+    __shared__ int s_top[4][kN];       // each softmax warp's maximum, or sum
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
     auto bar = [&](int which) { return base + L::kBarsAt + 8u * which; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -178,28 +126,20 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         tc::mbar_wait(bar(which), phase & 1, dead);
         __syncwarp();
     };
-    auto warp_arrive = [&](int which) {
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(which));
-    };
 
     if (tid == 0) {
         s_dead = 0;
-        tc::mbar_init(bar(kFullLow), 16);
-        tc::mbar_init(bar(kFullHigh), 16 + 2);
-        tc::mbar_init(bar(kLowHere), 64);
-        tc::mbar_init(bar(kLowRead), 16);
-        tc::mbar_init(bar(kHighHere), 64);
-        tc::mbar_init(bar(kHighRead), 16);
+        tc::mbar_init(bar(kFullLow), 8);
+        tc::mbar_init(bar(kFullHigh), 8);
         tc::mbar_init(bar(kFreeLow), 1);
         tc::mbar_init(bar(kOutput), 1);
         tc::mbar_init(bar(kScores), 1);
-        tc::mbar_init(bar(kWeights), 16);
-        tc::mbar_init(bar(kQuery), 16);
+        tc::mbar_init(bar(kWeights), 128);
+        tc::mbar_init(bar(kQuery), 128);
         tc::mbar_init(bar(kDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
+    if (warp == 12) tc::tmem_alloc<512>(tc::smem_u32(&s_tmem));
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -211,16 +151,86 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     const int32_t u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
     const int tiles = div.tiles;
 
-    if (warp == 16) {
+    if (warp >= 4 && warp < 12) {
+        // ---- rows: global memory -> registers -> dequantised blocks ----
+        // lane = 8 q + 2 rr + lp: row rr of four, latents 32 * (2 q + lp) .. of either half.  Eight
+        // consecutive lanes store to four rows x two chunks, which the swizzle spreads over all banks.
+        const int quarter = lane >> 3, lp = lane & 1;
+        const int row0 = (warp - 4) * 4 + ((lane >> 1) & 3);  // and row0 + 32, 64, 96
+        const int chunk = 2 * quarter + lp, rope_chunk = lp * 4 + quarter;
+        int32_t bits = 0;
+        uint4 low[4], high[4], rope[4];
+        uint32_t low_scales[4], high_scales[4];
+        int32_t slot[4];
+        Walk ahead(div, u0);
+        int token = ahead.row % op.tokens;
+        auto load_slots = [&] {
+            const int32_t* row = op.slots + token * op.slots_token;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = ahead.tile * kTile + i * 32 + row0;
+                slot[i] = ahead.u < u1 && e < op.topk ? __ldg(row + e) : kNotFound;
+            }
+        };
+        auto load_rows = [&] {
+            const uint8_t* pool = op.pool + static_cast<uint64_t>(token) * op.pool_token;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool there = slot[i] >= 0 && slot[i] < op.pool_rows;
+                if (!there && slot[i] != kNotFound) bits |= ASU_ST_BAD_QUERY;
+                const uint8_t* p = there ? pool + static_cast<uint64_t>(slot[i]) * op.pool_pitch
+                                         : reinterpret_cast<const uint8_t*>(g_zero_row);
+                low[i] = load16(p + chunk * 16);
+                high[i] = load16(p + 128 + chunk * 16);
+                rope[i] = load16(p + kRopeOffset + rope_chunk * 16);
+                low_scales[i] = load2(p + kScaleOffset + chunk * 2);
+                high_scales[i] = load2(p + kScaleOffset + 16 + chunk * 2);
+            }
+        };
+        auto next = [&] {
+            const int row = ahead.row;
+            ahead.next(div);
+            if (ahead.row != row && ++token == op.tokens) token = 0;
+        };
+        load_slots();
+        load_rows();
+        next();
+        load_slots();
+        const uint32_t at = base + L::kRows + quarter * kBlock + row0 * 128 + (((lp * 4) ^ (row0 & 7)) << 4);
+        const uint32_t rope_at = base + L::kRope + row0 * 128 + ((rope_chunk ^ (row0 & 7)) << 4);
+        const uint32_t count = u1 - u0;
+        for (uint32_t n = 0; n < count; ++n) {
+            if (n >= 1) warp_wait(kFreeLow, n - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dequantise(low[i], low_scales[i], at + i * 32 * 128);
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(bar(kFullLow));
+            if (n >= 1) warp_wait(kOutput, n - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dequantise(high[i], high_scales[i], at + 4 * kBlock + i * 32 * 128);
+                shared_store16(rope_at + i * 32 * 128, rope[i].x, rope[i].y, rope[i].z, rope[i].w);
+            }
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(bar(kFullHigh));
+            load_rows();
+            next();
+            load_slots();
+        }
+        if (bits) flag_status(op.status, 0, bits);
+    } else if (warp == 12) {
         // ---- the products, all by one lane.  (The branch has to be that of elect.sync itself: with a plain
         // lane number, or its result kept, the issue of a product takes 80 cycles instead of 30.) ----
         if (tc::elect_one()) {
             constexpr uint32_t kDescS = tc::instruction(128, kN, false, false);
             constexpr uint32_t kDescO = tc::instruction(128, kN, true, true);
+            constexpr uint32_t kHigh = tc::operand_high(128);
             const uint32_t desc_q = tc::operand(base + L::kQ, 0);
             const uint32_t desc_k = tc::operand(base + L::kRows, 0);
             const uint32_t desc_v = tc::operand(base + L::kRows, kBlock);
-            const uint32_t desc_p = tc::operand(base + L::kP, 0);
+            const uint32_t desc_p = tc::operand(base + L::kRope, 0);
             auto wait = [&](int which, uint32_t phase) { tc::mbar_wait(bar(which), phase & 1, dead); };
             uint32_t n = 0, segment = 0;
             for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
@@ -235,7 +245,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                         if (i == 4 && part == 0) continue;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            tc::mma_ss<tc::operand_high(128), tc::operand_high(128)>(
+                            tc::mma_ss<kHigh, kHigh>(
                                 L::kColS, desc_k + (4 * part + i) * (kBlock / 16) + 2 * k,
                                        desc_q + (4 * part + i) * (L::kQBlock / 16) + 2 * k, kDescS, part || i || k);
                     }
@@ -247,251 +257,170 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 for (int t = 0; t < 4; ++t) {
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc::mma_ss<tc::operand_high(128), tc::operand_high(L::kWeightRow)>(
-                            t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * L::kWeightRow, kDescO,
-                            !first || k);
+                        tc::mma_ss<kHigh, kHigh>(t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * (2048 / 16), kDescO,
+                                   !first || k);
                     if (t == 1) tc::commit(bar(kFreeLow));
                 }
                 tc::commit(bar(kOutput));
             }
         }
         __syncwarp();
-    } else if (warp > 16) {
-        // ---- rows: asynchronous copies, a tile ahead; a warp 64 rows of it.  An entry that is not there copies
-        // nothing and leaves zeros: finite values, whose weights are 0. ----
-        const int row0 = (warp - 17) * 64;
-        int32_t bits = 0;
-        Walk at(div, u0);
-        int token = at.row % op.tokens;
-        int32_t slot[2];
-        auto load_slots = [&] {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int e = at.tile * kTile + row0 + i * 32 + lane;
-                slot[i] = at.u < u1 && e < op.topk ? __ldg(op.slots + token * op.slots_token + e) : kNotFound;
-            }
-        };
-        load_slots();
-        // 9 lanes a row and half: 8 chunks of nibbles, swizzled, and the scales
-        const int lane_row = lane / 9, piece = lane - lane_row * 9;
-        const uint32_t rope = base + L::kRope + (row0 + (lane >> 3)) * 128;
-        const uint32_t count = u1 - u0;
-        for (uint32_t n = 0; n < count; ++n) {
-            const uint64_t pool = reinterpret_cast<uint64_t>(op.pool) + static_cast<uint64_t>(token) * op.pool_token;
-            uint64_t from[2];
-            uint32_t valid[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool there = slot[i] >= 0 && slot[i] < op.pool_rows;
-                if (!there && slot[i] != kNotFound) bits |= ASU_ST_BAD_QUERY;
-                valid[i] = __ballot_sync(0xffffffffu, there);
-                from[i] = pool + static_cast<uint64_t>(there ? slot[i] : 0) * op.pool_pitch;
-            }
-            const int row = at.row;
-            at.next(div);
-            if (at.row != row && ++token == op.tokens) token = 0;
-            load_slots();
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                if (n >= 1) warp_wait(half ? kHighRead : kLowRead, n - 1);
-                const uint32_t raw = base + L::kRaw + half * kRawHalf;
-                const int offset = piece < 8 ? half * 128 + piece * 16 : kScaleOffset + half * 16;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int r = 0; r < 33; r += 3) {
-                        const int mine = r + lane_row;
-                        const uint64_t src = __shfl_sync(0xffffffffu, from[i], mine & 31) + offset;
-                        const int to_row = row0 + i * 32 + mine;
-                        const uint32_t to = raw + (piece < 8 ? to_row * 128 + ((piece ^ (to_row & 7)) << 4)
-                                                             : kTile * 128 + to_row * 16);
-                        if (lane < 27 && mine < 32)
-                            copy16(to, reinterpret_cast<const void*>(src), (valid[i] >> (mine & 31)) & 1u);
-                    }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar(half ? kHighHere : kLowHere))
-                             : "memory");
-            }
-            if (n >= 1) warp_wait(kScores, n - 1);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 32; r += 4) {  // 8 lanes a row, into the swizzled block
-                    const int mine = r + (lane >> 3);
-                    const uint64_t src = __shfl_sync(0xffffffffu, from[i], mine) + kRopeOffset + (lane & 7) * 16;
-                    copy16(rope + (i * 32 + r) * 128 + (((lane ^ mine) & 7) << 4), reinterpret_cast<const void*>(src),
-                           (valid[i] >> mine) & 1u);
-                }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            tc::fence_async_shared();
-            warp_arrive(kFullHigh);
-        }
-        if (bits) flag_status(op.status, 0, bits);
     } else {
-        // ---- rows: lane = 8 q + 2 rr + lp has row rr of four, latents 32 * (2 q + lp) .. of either half.  Eight
-        // consecutive lanes read and store four rows x two chunks: all banks, on both sides (a row is 72 words, 8
-        // more than a multiple of 32, and the blocks are swizzled). ----
-        const int quarter = lane >> 3, lp = lane & 1;
-        const int row0 = warp * 4 + ((lane >> 1) & 3);  // and row0 + 64
-        const int chunk = 2 * quarter + lp;
-        const uint32_t raw = base + L::kRaw + row0 * 128 + ((chunk ^ (row0 & 7)) << 4);
-        const uint32_t raw_scales = base + L::kRaw + kTile * 128 + row0 * 16 + chunk * 2;
-        const uint32_t rows_at = base + L::kRows + quarter * kBlock + row0 * 128 + (((lp * 4) ^ (row0 & 7)) << 4);
-        auto dequantise_half = [&](int half) {
-            uint4 code[2];
-            uint32_t scales[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                code[i] = shared_load16(raw + half * kRawHalf + i * 64 * 128);
-                scales[i] = shared_load2(raw_scales + half * kRawHalf + i * 64 * 16);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) dequantise(code[i], scales[i], rows_at + half * 4 * kBlock + i * 64 * 128);
-            tc::fence_async_shared();
-        };
-        // ---- softmax: this thread's entry of the tile, and its warp's heads ----
-        constexpr int kC = kN / 4;
-        const int part = warp >> 2;   // heads part * kC ..; of the output, latents part * 128 ..
-        const int entry = (warp & 3) * 32 + lane;
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        float l[kC];  // the entries' weights by head
-        // the row of work's q, zero for heads beyond the last: 8 lanes a block of a head
-        auto copy_q = [&](int row) {
+        // ---- softmax: a thread an entry of the tile; for the output, a thread a latent of 128 ----
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        auto softmax_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // these four warps
+        auto load_q = [&](int row) {
             const int token = row % op.tokens, head0 = row / op.tokens * kN;
-            const int h = tid >> 3;
-            if (h < kN) {
+            const __nv_bfloat16* q = op.q + token * op.q_token + (tid & 7) * 8;
+            const uint32_t to0 = base + L::kQ + (((tid ^ (tid >> 3)) & 7) << 4);
+#pragma unroll 1
+            for (int h = tid >> 3; h < kN; h += 16) {
                 const bool there = head0 + h < op.heads;
-                const __nv_bfloat16* from = op.q + token * op.q_token + (there ? head0 + h : 0) * op.q_head + (tid & 7) * 8;
-                const uint32_t to = base + L::kQ + h * 128 + (((tid ^ h) & 7) << 4);
+                const __nv_bfloat16* from = q + (there ? head0 + h : 0) * op.q_head;
                 if (op.q_aligned || !there) {
 #pragma unroll
-                    for (int k = 0; k < 9; ++k) copy16(to + k * L::kQBlock, from + k * 64, there);
+                    for (int k = 0; k < 9; ++k)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to0 + k * L::kQBlock + h * 128),
+                                     "l"(from + k * 64), "r"(there ? 16 : 0)
+                                     : "memory");
                 } else {
 #pragma unroll 1
                     for (int k = 0; k < 9; ++k) {
                         const uint4 v = load_unaligned(from + k * 64);
-                        shared_store16(to + k * L::kQBlock, v.x, v.y, v.z, v.w);
+                        shared_store16(to0 + k * L::kQBlock + h * 128, v.x, v.y, v.z, v.w);
                     }
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc::fence_async_shared();
+            tc::mbar_arrive(bar(kQuery));
         };
-
+        constexpr int kC = kN < 32 ? kN : 32;  // columns at a time
+        float l[kN];                           // this thread's entries' weights by head
         Walk at(div, u0);
+        load_q(at.row);
         int token = at.row % op.tokens;
-        copy_q(at.row);
-        auto slot_here = [&]() -> int32_t {
-            const int e = at.tile * kTile + entry;
-            return at.u < u1 && e < op.topk ? __ldg(op.slots + token * op.slots_token + e) : kNotFound;
+        auto slot_here = [&](const Walk& w, int tok) -> bool {
+            const int e = w.tile * kTile + tid;
+            if (w.u >= u1 || e >= op.topk) return false;
+            const int32_t s = __ldg(op.slots + tok * op.slots_token + e);
+            return s >= 0 && s < op.pool_rows;
         };
-        int32_t slot = slot_here();
+        bool there = slot_here(at, token);
         for (uint32_t n = 0; at.u < u1; ++n) {
             const int row = at.row, tile = at.tile;
             const bool first = at.u == u0 || tile == 0;
             const bool last = at.u + 1 == u1 || tile + 1 == tiles;
-            const bool there = slot >= 0 && slot < op.pool_rows;
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                warp_wait(half ? kHighHere : kLowHere, n);
-                if (n >= 1) warp_wait(half ? kOutput : kFreeLow, n - 1);
-                dequantise_half(half);
-                __syncwarp();
-                if (lane == 0) {
-                    tc::mbar_arrive(bar(half ? kFullHigh : kFullLow));
-                    tc::mbar_arrive(bar(half ? kHighRead : kLowRead));
-                }
-            }
-            if (first) {  // q is on its way since the piece before
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                tc::fence_async_shared();
-                warp_arrive(kQuery);
+            if (first) {
 #pragma unroll
-                for (int h = 0; h < kC; ++h) l[h] = 0.0f;
+                for (int h = 0; h < kN; ++h) l[h] = 0.0f;
             }
             warp_wait(kScores, n);
+            if (n >= 1) warp_wait(kOutput, n - 1);  // long done: these scores came after it
             tc::fence_after();
-            uint32_t s[kC];
-            tc::tmem_load(lanes + L::kColS + part * kC, s);
-            tc::tmem_wait_load(s);
             // does a score exceed its reference by too much?
-            float minus_ref[kC];
             bool over = false;
             if (!first) {
-                load_shared(minus_ref, s_minus_ref + part * kC);
+#pragma unroll 1
+                for (int c0 = 0; c0 < kN; c0 += kC) {
+                    uint32_t s[kC];
+                    tc::tmem_load(lanes + L::kColS + c0, s);
+                    tc::tmem_wait_load(s);
+                    float top = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < kC; ++h)
-                    over |= fmaf(__uint_as_float(s[h]), op.scale_log2, minus_ref[h]) > kMaxGrowth;
+                    for (int h = 0; h < kC; ++h)
+                        top = fmaxf(top, fmaf(__uint_as_float(s[h]), op.scale_log2, s_minus_ref[c0 + h]));
+                    over |= top > kMaxGrowth;
+                }
                 over &= there;
             }
-            if (tc::any_of<kWorkers>(over || first)) {
+            if (tc::any_of<128>(over || first)) {
                 // new references: the maxima over the tile's entries, of this tile alone in a piece's first
+#pragma unroll 1
+                for (int c0 = 0; c0 < kN; c0 += kC) {
+                    uint32_t s[kC];
+                    tc::tmem_load(lanes + L::kColS + c0, s);
+                    tc::tmem_wait_load(s);
 #pragma unroll
-                for (int h = 0; h < kC; ++h) {
-                    const float x = there ? __uint_as_float(s[h]) * op.scale_log2 : -INFINITY;
-                    const int top = __reduce_max_sync(0xffffffffu, ordered(x));
-                    if (lane == h) s_top[warp & 3][part * kC + h] = top;
+                    for (int h = 0; h < kC; ++h) {
+                        const float x = there ? __uint_as_float(s[h]) * op.scale_log2 : -INFINITY;
+                        const int top = __reduce_max_sync(0xffffffffu, ordered(x));
+                        if (lane == h) s_top[warp][c0 + h] = top;
+                    }
                 }
-                workers_sync();
+                softmax_sync();
                 if (tid < kN) {
                     const float top = unordered(max(max(s_top[0][tid], s_top[1][tid]), max(s_top[2][tid], s_top[3][tid])));
-                    // while all entries of a piece were missing there is no reference: +inf here, so that
-                    // the next score of any size exceeds it
+                    // a piece whose entries so far are all missing has reference "none": minus it is +inf here,
+                    // so that the next score of any size exceeds it
                     const float old = first ? INFINITY : s_minus_ref[tid];
                     const float now = fminf(old, -top);
                     s_fade[tid] = old == now ? 1.0f : old == INFINITY ? 0.0f : exp2_fast(now - old);
                     s_minus_ref[tid] = now;
                 }
-                workers_sync();
-                load_shared(minus_ref, s_minus_ref + part * kC);
+                softmax_sync();
                 if (!first) {
 #pragma unroll
-                    for (int h = 0; h < kC; ++h) l[h] *= s_fade[part * kC + h];
+                    for (int h = 0; h < kN; ++h) l[h] *= s_fade[h];
 #pragma unroll 1
-                    for (int c0 = 0; c0 < kN; c0 += 16) {
-                        uint32_t o[16];
-                        tc::tmem_load(lanes + part * kN + c0, o);
+                    for (int c0 = 0; c0 < 4 * kN; c0 += kC) {
+                        uint32_t o[kC];
+                        tc::tmem_load(lanes + c0, o);
                         tc::tmem_wait_load(o);
 #pragma unroll
-                        for (int h = 0; h < 16; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * s_fade[c0 + h]);
-                        tc::tmem_store(lanes + part * kN + c0, o);
+                        for (int h = 0; h < kC; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * s_fade[(c0 + h) % kN]);
+                        tc::tmem_store(lanes + c0, o);
                     }
                     tc::tmem_wait_store();
                 }
             }
             const int64_t unit = static_cast<int64_t>(row) * tiles + tile;
-            uint32_t p[kC / 2];
+            if (op.weights != nullptr && tid < kN) scratch.ref[unit * kN + tid] = -s_minus_ref[tid];
 #pragma unroll
-            for (int h = 0; h < kC; h += 2) {
-                float a = exp2_fast(fmaf(__uint_as_float(s[h]), op.scale_log2, minus_ref[h]));
-                float b = exp2_fast(fmaf(__uint_as_float(s[h + 1]), op.scale_log2, minus_ref[h + 1]));
-                a = there ? a : 0.0f;
-                b = there ? b : 0.0f;
-                l[h] += a;
-                l[h + 1] += b;
-                p[h / 2] = pack_bf16(a, b);
+            for (int c0 = 0; c0 < kN; c0 += kC) {
+                uint32_t s[kC];
+                tc::tmem_load(lanes + L::kColS + c0, s);
+                tc::tmem_wait_load(s);
+                uint32_t p[kC / 2];
+#pragma unroll
+                for (int h = 0; h < kC; h += 2) {
+                    float a = exp2_fast(fmaf(__uint_as_float(s[h]), op.scale_log2, s_minus_ref[c0 + h]));
+                    float b = exp2_fast(fmaf(__uint_as_float(s[h + 1]), op.scale_log2, s_minus_ref[c0 + h + 1]));
+                    a = there ? a : 0.0f;
+                    b = there ? b : 0.0f;
+                    l[c0 + h] += a;
+                    l[c0 + h + 1] += b;
+                    p[h / 2] = pack_bf16(a, b);
+                }
+                const uint32_t to = base + L::kRope + tid * 128;
+#pragma unroll
+                for (int i = 0; i < kC / 8; ++i)
+                    shared_store16(to + (((c0 / 8 + i) ^ (tid & 7)) << 4), p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+                if (op.weights != nullptr) {
+                    uint4* out = reinterpret_cast<uint4*>(scratch.p + (unit * kTile + tid) * kN + c0);
+#pragma unroll
+                    for (int i = 0; i < kC / 8; ++i) out[i] = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+                }
             }
-            store_weights(base + L::kP, entry, part, p);
             tc::fence_async_shared();
             tc::fence_before();
-            warp_arrive(kWeights);
-            if (op.weights != nullptr) {
-                store_weights(scratch.p + (unit * kTile + entry) * kN + part * kC, p);
-                if (entry < kC) scratch.ref[unit * kN + part * kC + entry] = -s_minus_ref[part * kC + entry];
-            }
+            tc::mbar_arrive(bar(kWeights));
             at.next(div);
             const int was = token;
             if (at.row != row && ++token == op.tokens) token = 0;
-            slot = slot_here();
+            there = slot_here(at, token);
             if (last) {
                 // this row's scores are all made: the next one's q comes beside the output products
-                if (at.u < u1) copy_q(at.row);
-                // sums over the entries: within the warps, then the four quarters
+                if (at.u < u1) load_q(at.row);
+                // sums over the entries: within the warps, then the four
 #pragma unroll
-                for (int h = 0; h < kC; ++h) {
+                for (int h = 0; h < kN; ++h) {
                     float x = l[h];
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-                    if (lane == h) s_top[warp & 3][part * kC + h] = __float_as_int(x);
+                    if (lane == (h & 31)) s_top[warp][h] = __float_as_int(x);
                 }
-                workers_sync();
+                softmax_sync();
                 const int head0 = row / op.tokens * kN;
                 const int row_start = row * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
@@ -509,22 +438,25 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                         scratch.ml[(piece * 2 + 1) * kN + tid] = sum;
                     }
                 }
-                workers_sync();
+                softmax_sync();
                 warp_wait(kOutput, n);
                 tc::fence_after();
-                const int latent = part * 128 + entry;
-                __nv_bfloat16* out = op.out + (static_cast<int64_t>(was) * op.heads + head0) * kLatent + latent;
-                float* partial = scratch.o + static_cast<int64_t>(piece) * kN * kLatent + latent;
 #pragma unroll 1
-                for (int c0 = 0; c0 < kN; c0 += 16) {
-                    uint32_t o[16];
-                    tc::tmem_load(lanes + part * kN + c0, o);
+                for (int c0 = 0; c0 < 4 * kN; c0 += kC) {
+                    uint32_t o[kC];
+                    tc::tmem_load(lanes + c0, o);
                     tc::tmem_wait_load(o);
+                    const int latent = c0 / kN * 128 + tid, h0 = c0 % kN;
+                    if (whole) {
+                        __nv_bfloat16* to = op.out + (static_cast<int64_t>(was) * op.heads + head0 + h0) * kLatent + latent;
 #pragma unroll
-                    for (int h = 0; h < 16; ++h) {
-                        if (!whole) partial[(c0 + h) * kLatent] = __uint_as_float(o[h]);
-                        else if (head0 + c0 + h < op.heads)
-                            out[(c0 + h) * kLatent] = __float2bfloat16(__uint_as_float(o[h]) * s_fade[c0 + h]);
+                        for (int h = 0; h < kC; ++h)
+                            if (head0 + h0 + h < op.heads)
+                                to[h * kLatent] = __float2bfloat16(__uint_as_float(o[h]) * s_fade[h0 + h]);
+                    } else {
+                        float* to = scratch.o + (static_cast<int64_t>(piece) * kN + h0) * kLatent + latent;
+#pragma unroll
+                        for (int h = 0; h < kC; ++h) to[h * kLatent] = __uint_as_float(o[h]);
                     }
                 }
                 tc::fence_before();
@@ -534,7 +466,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     pdl_trigger();
     __syncthreads();
     if (s_dead && tid == 0) flag_status(op.status, 0, ASU_ST_TIMEOUT);
-    if (warp == 16) {
+    if (warp == 12) {
         // Nothing of this block may be in flight when its tensor memory goes and its barriers with it,
         // whatever way the loops were left.
         if (tc::elect_one()) {
@@ -634,9 +566,7 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
     op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(w);
 }
 
-int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
-
-int columns_of(int64_t heads) { return heads <= 16 ? 16 : 32; }
+int columns_of(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
 Division division(int64_t tokens, int64_t heads, int64_t topk, int sms) {
     const int n = columns_of(heads);
@@ -676,14 +606,18 @@ int launch(cudaStream_t s, const Operands& op, void* workspace) {
 
 }  // namespace
 
-int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+int64_t tall_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
     int64_t at[5];
     layout(division(tokens, heads, topk, asu_sm_count()), columns_of(heads), weights, at);
     return at[4];
 }
 
-int launch_decode(cudaStream_t s, const Operands& op, void* workspace) {
-    return columns_of(op.heads) == 16 ? launch<16>(s, op, workspace) : launch<32>(s, op, workspace);
+int launch_tall(cudaStream_t s, const Operands& op, void* workspace) {
+    switch (columns_of(op.heads)) {
+        case 16: return launch<16>(s, op, workspace);
+        case 32: return launch<32>(s, op, workspace);
+        default: return launch<64>(s, op, workspace);
+    }
 }
 
 }  // namespace kv4

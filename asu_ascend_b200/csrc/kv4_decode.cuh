@@ -79,9 +79,62 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return reinterpret_cast<const uint32_t&>(v);
 }
 
-// kv4_decode.cu
-int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
-int launch_decode(cudaStream_t stream, const Operands& op, void* workspace);
+__device__ __forceinline__ void shared_store16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// 32 latents as four 16-byte chunks of a swizzled row; chunk i goes to `at` with i in address bits 4 and 5.
+__device__ __forceinline__ void dequantise(const uint4& code, uint32_t scales, uint32_t at) {
+    const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_bfloat162 s, c;
+        scale_pair(scales, i / 2, s, c);
+        uint32_t v[4];
+        unpack_word(w[i], s, c, v);
+        shared_store16(at ^ (i << 4), v[0], v[1], v[2], v[3]);
+    }
+}
+
+// 8 values that start on any element.
+__device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
+    uint32_t w[4];
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = static_cast<uint32_t>(__ldg(s + 2 * i)) | (static_cast<uint32_t>(__ldg(s + 2 * i + 1)) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Pairs of floats in one register pair: one instruction for two.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// kv4_decode.cu: up to kTallHeads heads
+constexpr int kTallHeads = 64;
+int64_t tall_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
+int launch_tall(cudaStream_t stream, const Operands& op, void* workspace);
+// kv4_decode_wide.cu: more
+int64_t wide_workspace(int64_t tokens, int64_t topk, bool weights);
+int launch_wide(cudaStream_t stream, const Operands& op, void* workspace);
 
 }  // namespace kv4
 }  // namespace asu

@@ -164,6 +164,16 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint3
         "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHighA), "n"(kHighB)
         : "memory");
 }
+// A in tensor memory: a lane a row of M, a column two values of K.
+template <uint32_t kHighB>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; .reg .b64 y; setp.ne.u32 p, %4, 0;\n"
+        "mov.b64 y, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHighB)
+        : "memory");
+}
 // The barrier completes when every tcgen05.mma issued by this thread so far has.
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
