@@ -8,15 +8,18 @@
 //   resolve: a resident key is a hit; the first occurrence of a missing key pops the stack (top
 //       first, in query order), later ones are hits; an empty stack leaves slot -1
 //
-// One CTA of 1024 threads per row.  Thread t owns the slots [t * IPT_S, (t + 1) * IPT_S) and keeps
-// their scores and keys in registers, so that ranks in slot order come from a block scan and the row
-// is read and written once.  A request's step is a serial chain of block barriers over a few dozen
-// KB: latency-bound, not bandwidth-bound.
-//  * Scores are sums of non-negative floats, whose bit patterns order like integers.  The E-th
-//    lowest is found bit by bit from the top: 31 block-wide counts of "below the trial value".
-//    No sort and no histogram; the result does not depend on scheduling.
-//  * Ties at the threshold go to the lower slots: one packed scan ranks the slots below it
-//    and the ties together.
+// One CTA of 1024 threads per row.  A request's step is a serial chain of dependent loads and block barriers
+// over a few dozen KB: latency-bound, not bandwidth-bound.
+//  * A warp owns a run of slots and takes 32 of them at a time: loads are of whole lines, shared memory has
+//    no bank conflicts, and ranks in slot order need the ballots and one exchange of a count per warp.
+//    (With a run of slots for each thread, strided, and a sum over the block for every bit of the
+//    threshold, the step took 51 us for 10240 slots and 36 us for 8192.)
+//  * Scores are sums of non-negative floats, whose bit patterns order like integers.  The E-th lowest is
+//    found by three counts of digits, of 11, 11 and 9 bits, and fewer when a digit's slots leave all.
+//    Counts are integers: the result does not depend on scheduling.
+//  * Ties at the threshold go to the lower slots.
+//  * A slot that the last step names several times gets its weights in their order: each round of
+//    additions takes the first entry that is left of every slot.
 //  * The products and sums of U are rounded one by one (no fma), so that a plain
 //    decay-then-add gives the same bits and the same victims.
 #include "asu_common.cuh"
@@ -28,21 +31,13 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int32_t kEmptyKey = -1;
+constexpr int kBins = 2048;  // of the first two digits; 512 of the last
+constexpr int kHistogram = 2 * kBins + 512;
 
 enum : uint8_t { kInvalid = 0, kHit = 1, kMiss = 2, kBad = 3 };
 
 __device__ __forceinline__ uint32_t hash_slot(int32_t key, int log2h) {
     return (static_cast<uint32_t>(key) * 0x9E3779B1u) >> (32 - log2h);
-}
-
-// Sum of one small count per thread over the block; `buf` holds 32 ints.  One barrier: alternate two
-// buffers between back-to-back calls.
-__device__ __forceinline__ int block_sum_1b(int v, int* buf) {
-    const int lane = threadIdx.x & 31;
-    v = __reduce_add_sync(0xffffffffu, v);
-    if (lane == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, buf[lane]);
 }
 
 __device__ __forceinline__ float weight_at(const void* w, int dtype, uint64_t i) {
@@ -51,6 +46,14 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, uint64_t i)
     return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
 
+// Sum of the warps' values before this warp, and of all.
+__device__ __forceinline__ int before_warp(const int* per_warp, int* total) {
+    const int lane = threadIdx.x & 31, v = per_warp[lane];
+    *total = __reduce_add_sync(0xffffffffu, v);
+    return __reduce_add_sync(0xffffffffu, lane < static_cast<int>(threadIdx.x >> 5) ? v : 0);
+}
+
+// IPT_Q: keys, and entries of the last step, a thread at most; IPT_S: slots.
 template <int IPT_Q, int IPT_S>
 __global__ void __launch_bounds__(kThreads)
 weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* __restrict__ score,
@@ -62,23 +65,30 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
                    uint32_t K, uint32_t S, uint32_t Q, uint32_t target, int log2h) {
     pdl_wait();
     pdl_trigger();
-    extern __shared__ int32_t smem[];
+    extern __shared__ __align__(16) int32_t smem[];
     const uint32_t H = 1u << log2h;
-    float* s_sum = reinterpret_cast<float*>(smem);          // [S] decayed score + weights
-    int32_t* s_claim = smem + S;                            // [S] first entry naming the slot; later the victims
+    int32_t* s_count = smem;                                // [kHistogram] candidates by digit
+    float* s_sum = reinterpret_cast<float*>(smem + kHistogram);  // [S] decayed score + weights
+    int32_t* s_claim = smem + kHistogram + S;               // [S] first entry left that names the slot; later the victims
     int32_t* s_hkey = s_claim + S;                          // [H] hash: key
     int32_t* s_hpos = s_hkey + H;                           // [H] hash: first position of the key
     int32_t* s_hval = s_hpos + H;                           // [H] hash: installed slot
     uint8_t* s_asked = reinterpret_cast<uint8_t*>(s_hval + H);  // [S] a key of this step is in the slot
-    __shared__ int buf_a[32], buf_b[32];
-    __shared__ int n_hits, n_valid, n_double;
-    const int tid = threadIdx.x;
+    __shared__ int buf_a[32], buf_b[32], buf_q[32];
+    __shared__ int n_hits, n_valid;
+    __shared__ int s_digit[3];  // of the threshold; candidates below it; in it
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t below_lane = (1u << lane) - 1;
     const uint32_t r = blockIdx.x;
     int32_t* trow = t2s + static_cast<uint64_t>(r) * K;
     int32_t* srow = s2t + static_cast<uint64_t>(r) * S;
     float* crow = score + static_cast<uint64_t>(r) * S;
     int32_t* krow = stack + static_cast<uint64_t>(r) * S;
     int32_t bits = 0;
+    // the warp's keys, entries and slots: item j of the lane
+    const int per_q = (Q + kThreads - 1) / kThreads, per_s = (S + kThreads - 1) / kThreads;
+    auto pos_of = [&](int j) { return static_cast<uint32_t>((warp * per_q + j) * 32 + lane); };
+    auto slot_of = [&](int j) { return static_cast<uint32_t>((warp * per_s + j) * 32 + lane); };
 
     // ---- loads; shared-memory set-up ----
     const int32_t free0 = ld_cg(count + r);
@@ -86,31 +96,36 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
     int32_t key[IPT_Q], g[IPT_Q];
 #pragma unroll
     for (int j = 0; j < IPT_Q; ++j) {
-        const uint32_t pos = tid + j * kThreads;
         key[j] = -1;
-        g[j] = kNotFound;
-        if (pos < Q) {
-            key[j] = __ldg(query + static_cast<uint64_t>(r) * Q + pos);
-            if (static_cast<uint32_t>(key[j]) < K) g[j] = ld_cg(trow + key[j]);
-        }
+        if (j < per_q && pos_of(j) < Q) key[j] = __ldg(query + static_cast<uint64_t>(r) * Q + pos_of(j));
+    }
+    const uint64_t last_row = static_cast<uint64_t>(r) * last_count;
+    int32_t named[IPT_Q];  // the entries' slots
+    float w[IPT_Q];        // and weights
+#pragma unroll
+    for (int j = 0; j < IPT_Q; ++j) {
+        const uint32_t p = tid + j * kThreads;
+        named[j] = p < last_count ? __ldcg(last_slot + last_row + p) : kNotFound;
+        w[j] = p < last_count ? weight_at(last_weight, weight_dtype, last_row + p) : 0.0f;
     }
     int32_t owner[IPT_S];
+    float faded[IPT_S];
 #pragma unroll
     for (int j = 0; j < IPT_S; ++j) {
-        const uint32_t s = tid * IPT_S + j;
-        owner[j] = kNotFound;
-        if (s < S) {
-            owner[j] = ld_cg(srow + s);
-            s_sum[s] = __fmul_rn(__ldcg(crow + s), decay);
-            s_claim[s] = INT32_MAX;
-            s_asked[s] = 0;
-        }
+        const bool mine = j < per_s && slot_of(j) < S;
+        owner[j] = mine ? ld_cg(srow + slot_of(j)) : kNotFound;
+        faded[j] = mine ? __ldcg(crow + slot_of(j)) : 0.0f;
     }
     for (uint32_t i = tid; i < H; i += kThreads) {
         s_hkey[i] = kEmptyKey;
         s_hpos[i] = INT32_MAX;
     }
-    if (tid == 0) n_hits = n_valid = n_double = 0;
+    for (uint32_t i = tid; i < kHistogram; i += kThreads) s_count[i] = 0;
+    for (uint32_t i = tid; i < S; i += kThreads) {
+        s_claim[i] = INT32_MAX;
+        s_asked[i] = 0;
+    }
+    if (tid == 0) n_hits = n_valid = 0;
     if (free0 < 0 || free0 > static_cast<int32_t>(S)) {  // uniform across the block
         if (tid == 0) {
             flag_status(status, r, ASU_ST_BAD_STATE);
@@ -123,24 +138,41 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
         }
         return;
     }
+#pragma unroll
+    for (int j = 0; j < IPT_Q; ++j)
+        g[j] = static_cast<uint32_t>(key[j]) < K ? ld_cg(trow + key[j]) : kNotFound;
+#pragma unroll
+    for (int j = 0; j < IPT_S; ++j) {
+        if (j >= per_s || slot_of(j) >= S) continue;
+        const float v = __fmul_rn(faded[j], decay);
+        if (!(v >= 0.0f) && owner[j] >= 0) bits |= ASU_ST_BAD_STATE;
+        s_sum[slot_of(j)] = v > 0.0f ? v : 0.0f;  // never -0: the bits are ordered as unsigned ones
+    }
     __syncthreads();
 
     // ---- the last step's entries claim their slots; this step's keys are classified ----
-    const uint64_t last_row = static_cast<uint64_t>(r) * last_count;
-    for (uint32_t p = tid; p < last_count; p += kThreads) {
-        const int32_t s = __ldcg(last_slot + last_row + p);
-        if (static_cast<uint32_t>(s) < S) atomicMin(&s_claim[s], static_cast<int32_t>(p));
-        else if (s != kNotFound) bits |= ASU_ST_BAD_QUERY;
+#pragma unroll
+    for (int j = 0; j < IPT_Q; ++j) {
+        if (static_cast<uint32_t>(named[j]) >= S) {
+            if (named[j] != kNotFound) bits |= ASU_ST_BAD_QUERY;
+            named[j] = kNotFound;
+            continue;
+        }
+        if (!(w[j] >= 0.0f) || w[j] == INFINITY) {
+            bits |= ASU_ST_BAD_WEIGHT;
+            named[j] = kNotFound;
+            continue;
+        }
+        atomicMin(&s_claim[named[j]], tid + j * kThreads);
     }
     uint8_t st[IPT_Q];
     int32_t hidx[IPT_Q];
     int valid_local = 0;
 #pragma unroll
     for (int j = 0; j < IPT_Q; ++j) {
-        const int32_t pos = tid + j * kThreads;
         st[j] = kInvalid;
         hidx[j] = -1;
-        if (static_cast<uint32_t>(pos) >= Q) continue;
+        if (j >= per_q || pos_of(j) >= Q) continue;
         if (static_cast<uint32_t>(key[j]) >= K) {
             bits |= ASU_ST_BAD_QUERY;
             continue;
@@ -158,7 +190,7 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
                 h = (h + 1) & (H - 1);
             }
             hidx[j] = static_cast<int32_t>(h);
-            atomicMin(&s_hpos[h], pos);
+            atomicMin(&s_hpos[h], static_cast<int32_t>(pos_of(j)));
         } else {
             st[j] = kBad;
             bits |= ASU_ST_BAD_STATE;
@@ -166,124 +198,142 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
     }
     __syncthreads();
 
-    // ---- weights onto the sums: only the first entry of a slot writes it ----
-    for (uint32_t p = tid; p < last_count; p += kThreads) {
-        const int32_t s = __ldcg(last_slot + last_row + p);
-        if (static_cast<uint32_t>(s) >= S) continue;
-        const float w = weight_at(last_weight, weight_dtype, last_row + p);
-        if (!(w >= 0.0f) || w == INFINITY) bits |= ASU_ST_BAD_WEIGHT;
-        if (s_claim[s] == static_cast<int32_t>(p)) {
-            if (w >= 0.0f && w < INFINITY) s_sum[s] = __fadd_rn(s_sum[s], w);
-        } else {
-            n_double = 1;
-        }
-    }
-    __syncthreads();
-    if (n_double) {  // uniform; a slot named more than once: its first entry adds the others in order
-        for (uint32_t p = tid; p < last_count; p += kThreads) {
-            const int32_t s = __ldcg(last_slot + last_row + p);
-            if (static_cast<uint32_t>(s) >= S || s_claim[s] != static_cast<int32_t>(p)) continue;
-            float u = s_sum[s];
-            for (uint32_t i = p + 1; i < last_count; ++i) {
-                if (__ldcg(last_slot + last_row + i) != s) continue;
-                const float w = weight_at(last_weight, weight_dtype, last_row + i);
-                if (w >= 0.0f && w < INFINITY) u = __fadd_rn(u, w);
+    // ---- weights onto the sums: a slot's entries one after the other, in as many rounds as a slot has ----
+    while (true) {
+        int left = 0;
+#pragma unroll
+        for (int j = 0; j < IPT_Q; ++j) {
+            const int32_t s = named[j];
+            if (s == kNotFound) continue;
+            if (s_claim[s] == tid + j * kThreads) {
+                s_sum[s] = __fadd_rn(s_sum[s], w[j]);
+                s_claim[s] = INT32_MAX;  // no entry's own: who reads it meanwhile stays for the next round
+                named[j] = kNotFound;
+            } else {
+                left = 1;
             }
-            s_sum[s] = u;
         }
+        if (!__syncthreads_or(left)) break;
+#pragma unroll
+        for (int j = 0; j < IPT_Q; ++j)
+            if (named[j] != kNotFound) atomicMin(&s_claim[named[j]], tid + j * kThreads);
         __syncthreads();
     }
 
     // ---- who leaves ----
     uint32_t u[IPT_S];
-    bool may[IPT_S];
-    int cand_local = 0;
+    uint32_t may = 0;  // bit j: the slot is a candidate
 #pragma unroll
     for (int j = 0; j < IPT_S; ++j) {
-        const uint32_t s = tid * IPT_S + j;
-        may[j] = false;
         u[j] = 0;
-        if (s < S && owner[j] >= 0) {
-            const float v = s_sum[s];
-            u[j] = __float_as_uint(v);
-            may[j] = !s_asked[s] && owner[j] < bound;
+        if (j >= per_s || slot_of(j) >= S) continue;
+        if (owner[j] >= 0) {
+            u[j] = __float_as_uint(s_sum[slot_of(j)]);
+            if (!s_asked[slot_of(j)] && owner[j] < bound) may |= 1u << j;
         }
-        cand_local += may[j];
     }
     const int32_t tgt = static_cast<int32_t>(target < S ? target : S);
     int32_t E = tgt > free0 ? tgt - free0 : 0;
-    uint32_t cut = 0;  // the E-th lowest U among the candidates
-    int below = 0;     // candidates under it
-    if (E > 0) {       // uniform
-        const int n = block_sum_1b(cand_local, buf_a);
-        if (E > n) E = n;
-        for (int b = 30; b >= 0; --b) {
-            const uint32_t trial = cut | (1u << b);
-            int c = 0;
+    uint32_t cut = 0, whole = 0;  // the E-th lowest U among the candidates; all under `whole` leave
+    int quota = 0;                // and so many of those at cut
+    if (E > 0) {                  // uniform
+        int below = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 20 : pass == 1 ? 9 : 0;
+            const int width = pass == 2 ? 9 : 11;
+            int32_t* bins = s_count + pass * kBins;
 #pragma unroll
-            for (int j = 0; j < IPT_S; ++j) c += may[j] && u[j] < trial;
-            c = block_sum_1b(c, (b & 1) ? buf_a : buf_b);
-            if (c < E) {
-                cut = trial;
-                below = c;
+            for (int j = 0; j < IPT_S; ++j)
+                if (((may >> j) & 1u) && (pass == 0 || (u[j] ^ cut) >> (shift + width) == 0))
+                    atomicAdd(&bins[(u[j] >> shift) & ((1u << width) - 1)], 1);
+            __syncthreads();
+            const int2 c = pass < 2 || tid < 256 ? reinterpret_cast<const int2*>(bins)[tid] : make_int2(0, 0);
+            int total;
+            const int before = below + block_exclusive_scan_1b(c.x + c.y, buf_a, &total);
+            if (pass == 0 && E > total) E = total;
+            if (E == 0) break;
+            if (before < E && E <= before + c.x + c.y) {  // one thread
+                const bool second = E > before + c.x;
+                s_digit[0] = 2 * tid + second;
+                s_digit[1] = before + (second ? c.x : 0);
+                s_digit[2] = second ? c.y : c.x;
+            }
+            __syncthreads();
+            cut |= static_cast<uint32_t>(s_digit[0]) << shift;
+            below = s_digit[1];
+            whole = cut;
+            quota = E - below;
+            if (quota == s_digit[2]) {  // they leave all
+                whole = cut + (1u << shift);
+                quota = 0;
+                break;
             }
         }
-        __syncthreads();
     }
-    bool gone[IPT_S];
+    uint32_t gone = 0;
     if (E > 0) {
-        int packed = 0;
-#pragma unroll
-        for (int j = 0; j < IPT_S; ++j)
-            packed += may[j] ? (u[j] < cut ? 1 : (u[j] == cut ? 1 << 16 : 0)) : 0;
-        int total = 0;
-        packed = block_exclusive_scan_1b(packed, buf_a, &total);
-        int rank = packed & 0xffff, ties = packed >> 16;
-        const int quota = E - below;
-        rank += min(ties, quota);
+        int mine = 0;  // of the warp: those under `whole`, and those at cut from bit 16 on
 #pragma unroll
         for (int j = 0; j < IPT_S; ++j) {
-            const int32_t s = tid * IPT_S + j;
-            const bool tie = may[j] && u[j] == cut;
-            gone[j] = may[j] && (u[j] < cut || (tie && ties < quota));
-            ties += tie;
-            if (!gone[j]) continue;
+            const bool can = (may >> j) & 1u;
+            mine += __popc(__ballot_sync(0xffffffffu, can && u[j] < whole));
+            if (quota > 0) mine += __popc(__ballot_sync(0xffffffffu, can && u[j] == cut)) << 16;
+        }
+        if (lane == 0) buf_b[warp] = mine;
+        __syncthreads();
+        int total;
+        int before = before_warp(buf_b, &total), ties = before >> 16;
+        before &= 0xffff;
+#pragma unroll
+        for (int j = 0; j < IPT_S; ++j) {
+            const bool can = (may >> j) & 1u;
+            const bool under = can && u[j] < whole, tie = quota > 0 && can && u[j] == cut;
+            const uint32_t all_under = __ballot_sync(0xffffffffu, under), all_ties = __ballot_sync(0xffffffffu, tie);
+            const int tie_rank = ties + __popc(all_ties & below_lane);
+            const int rank = before + __popc(all_under & below_lane) + min(tie_rank, quota);
+            before += __popc(all_under);
+            ties += __popc(all_ties);
+            if (!under && !(tie && tie_rank < quota)) continue;
+            const int32_t s = static_cast<int32_t>(slot_of(j));
+            gone |= 1u << j;
             s_claim[rank] = s;
             st_cg(krow + free0 + rank, s);
             evicted[static_cast<uint64_t>(r) * ev_stride + rank] = owner[j];
             if (static_cast<uint32_t>(owner[j]) < K) st_cg(trow + owner[j], kNotFound);
             else bits |= ASU_ST_BAD_STATE;
             st_cg(srow + s, kNotFound);
-            ++rank;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < IPT_S; ++j) gone[j] = false;
     }
 #pragma unroll
-    for (int j = 0; j < IPT_S; ++j) {
-        const uint32_t s = tid * IPT_S + j;
-        if (s < S) __stcg(crow + s, gone[j] || owner[j] < 0 ? 0.0f : __uint_as_float(u[j]));
-    }
+    for (int j = 0; j < IPT_S; ++j)
+        if (j < per_s && slot_of(j) < S)
+            __stcg(crow + slot_of(j), ((gone >> j) & 1u) || owner[j] < 0 ? 0.0f : __uint_as_float(u[j]));
     for (int i = E + tid; i < tgt; i += kThreads) evicted[static_cast<uint64_t>(r) * ev_stride + i] = kNotFound;
     if (tid == 0) ev_count[r] = E;
     const int32_t free1 = free0 + E;
-    __syncthreads();  // victims listed and unmapped
 
     // ---- first occurrences of missing keys pop the stack in query order ----
-    int32_t slot[IPT_Q];
-    bool first[IPT_Q], inst[IPT_Q];
-    int taken = 0;
+    uint32_t first = 0, inst = 0;
+    int firsts = 0;
 #pragma unroll
     for (int j = 0; j < IPT_Q; ++j) {
-        const int32_t pos = tid + j * kThreads;
-        first[j] = st[j] == kMiss && s_hpos[hidx[j]] == pos;
-        int total = 0;
-        const int before = block_exclusive_scan_1b(first[j], (j & 1) ? buf_a : buf_b, &total);
+        const bool f = st[j] == kMiss && s_hpos[hidx[j]] == static_cast<int32_t>(pos_of(j));
+        first |= static_cast<uint32_t>(f) << j;
+        firsts += __popc(__ballot_sync(0xffffffffu, f));
+    }
+    if (lane == 0) buf_q[warp] = firsts;
+    __syncthreads();  // victims listed and unmapped
+    int taken;
+    int before = before_warp(buf_q, &taken);
+    int32_t slot[IPT_Q];
+#pragma unroll
+    for (int j = 0; j < IPT_Q; ++j) {
+        const bool f = (first >> j) & 1u;
+        const uint32_t all = __ballot_sync(0xffffffffu, f);
         slot[j] = st[j] == kHit ? g[j] : kNotFound;
-        inst[j] = false;
-        if (first[j]) {
-            const int32_t k = taken + before;
+        if (f) {
+            const int32_t k = before + __popc(all & below_lane);
             int32_t s = kNotFound;
             if (k < free1) {
                 s = k < E ? s_claim[E - 1 - k] : ld_cg(krow + (free0 - 1 - (k - E)));
@@ -295,37 +345,36 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
             if (s >= 0) {
                 st_cg(trow + key[j], s);
                 st_cg(srow + s, key[j]);
-                inst[j] = true;
+                inst |= 1u << j;
             } else {
                 bits |= ASU_ST_SHORTAGE;
             }
             s_hval[hidx[j]] = s;
             slot[j] = s;
         }
-        taken += total;
+        before += __popc(all);
     }
     const int32_t n_inst = taken < free1 ? taken : free1;
     __syncthreads();  // installed slots visible
     int hits_local = 0;
 #pragma unroll
     for (int j = 0; j < IPT_Q; ++j) {
-        const uint32_t pos = tid + j * kThreads;
         bool hit = st[j] == kHit;
-        if (st[j] == kMiss && !first[j]) {
+        if (st[j] == kMiss && !((first >> j) & 1u)) {
             slot[j] = s_hval[hidx[j]];
             hit = slot[j] >= 0;
         }
         hits_local += hit;
-        if (pos < Q) {
-            const uint64_t o = static_cast<uint64_t>(r) * Q + pos;
+        if (j < per_q && pos_of(j) < Q) {
+            const uint64_t o = static_cast<uint64_t>(r) * Q + pos_of(j);
             slot_out[o] = slot[j];
             hit_mask[o] = hit;
-            install_mask[o] = inst[j];
+            install_mask[o] = (inst >> j) & 1u;
         }
     }
     hits_local = __reduce_add_sync(0xffffffffu, hits_local);
     valid_local = __reduce_add_sync(0xffffffffu, valid_local);
-    if ((tid & 31) == 0) {
+    if (lane == 0) {
         if (hits_local) atomicAdd(&n_hits, hits_local);
         if (valid_local) atomicAdd(&n_valid, valid_local);
     }
@@ -363,10 +412,10 @@ int launch(cudaStream_t s, int32_t* t2s, int32_t* s2t, float* score, int32_t* st
     if (rc != ASU_OK) return rc;
     // hash load factor 1/2, or up to 1 where S and Q are both large (it still ends: Q <= H)
     int log2h = log2_ceil(2 * (Q < 16 ? 16 : Q));
-    size_t smem = 9ull * S + 12ull * (1ull << log2h);
+    size_t smem = 4ull * kHistogram + 9ull * S + 12ull * (1ull << log2h);
     if (smem > static_cast<size_t>(max_dynamic)) {
         --log2h;
-        smem = 9ull * S + 12ull * (1ull << log2h);
+        smem = 4ull * kHistogram + 9ull * S + 12ull * (1ull << log2h);
     }
     if (smem > static_cast<size_t>(max_dynamic)) return ASU_ERR_ARG;
     return launch_pdl(kernel, dim3(R), dim3(kThreads), smem, s, t2s, s2t, score, stack, count, last_slot, last_weight,
@@ -405,7 +454,7 @@ extern "C" int asu_weight_step(void* stream, int32_t* token_to_slot, int32_t* sl
     if (tgt > 0 && (evicted == nullptr || evicted_stride < tgt)) return ASU_ERR_ARG;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define ASU_WEIGHT_CASE(NQ, NS)                                                                                       \
-    if (query_count <= kThreads * NQ && slot_count <= kThreads * NS)                                                  \
+    if (query_count <= kThreads * NQ && last_count <= kThreads * NQ && slot_count <= kThreads * NS)                   \
         return launch<NQ, NS>(s, token_to_slot, slot_to_token, score, free_stack, free_count, last_slot, last_weight, \
                               weight_dtype, last_count, decay, keep_from, query, slot_out, hit_mask, install_mask,    \
                               evicted, evicted_stride, evicted_count, stats, status, req_num, key_space, slot_count,  \
