@@ -41,8 +41,8 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     const int64_t need = decode_workspace(tokens, heads, topk, weights != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_size < need)) return ASU_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(pool) % 16 || pool_pitch % 16 ||
-        pool_token_stride % 16 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(lse) % 4 ||
-        reinterpret_cast<uintptr_t>(workspace) % 16)
+        pool_token_stride % 16 || reinterpret_cast<uintptr_t>(out) % 32 || reinterpret_cast<uintptr_t>(lse) % 4 ||
+        reinterpret_cast<uintptr_t>(workspace) % 32)
         return ASU_ERR_ALIGN;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Operands op;

@@ -29,9 +29,12 @@ namespace {
 // The running maximum only moves when it grows by more than 2^8: until then the weights stay below
 // 2^8, as exact in bf16 as any others, and the output needs no rescaling.
 //
-// 128 tokens x 128 heads x 2048 entries take 130 us, with weights 164.  A tile takes 1.7 us, of which the
-// products are 1.1; a change of tokens 6 us (the next q's 147 KB, the output through the lanes), the start 6
-// us, and the joining of the pieces 10 to 20, with the weights' way through memory and back 30 more.
+// The two halves of a token follow one another, so that every other row of work finds its q in place.
+//
+// 128 tokens x 128 heads x 2048 entries take 122 us, with weights 143.  A tile takes 1.7 us, of which the
+// products are 1.0 and the traffic of shared memory 1.3; a change of tokens 6 us (the next q's 147 KB, the
+// output through the lanes), the start 6 us; the joining of the pieces 9, with the weights' way through memory
+// and back 23.
 constexpr int kTile = 64;  // entries a tile
 constexpr int kWideThreads = 15 * 32;
 constexpr int kBlock = kTile * 128;  // bytes of a [64 x 64] bf16 block
@@ -75,6 +78,12 @@ __device__ __forceinline__ uint4 shared_load16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
+}
+// A whole sector of a thread's own: nothing is gained by another thread's stores next to it.
+__device__ __forceinline__ void store32(void* to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 __device__ __forceinline__ uint32_t shared_load2(uint32_t at) {
     unsigned short v;
@@ -142,7 +151,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         uint32_t n = 0;
         for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
             const uint32_t raw = raw_at + (n & 1) * kRawTile;
-            const uint32_t mine = at.row >= op.tokens ? 8 : 0, other = 8 - mine;  // chunks before this half's
+            const uint32_t mine = at.row & 1 ? 8 : 0, other = 8 - mine;  // chunks before this half's
             warp_wait(bar2(kRowsHere, n), n >> 1);
             if (n >= 1) warp_wait(bar(kFreeA), n - 1);
 #pragma unroll
@@ -181,7 +190,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         auto slot_of = [&](const Walk& w) -> int32_t {
             const int e = w.tile * kTile + row0 + lane;
             if (w.u >= u1 || e >= op.topk) return kNotFound;
-            return __ldg(op.slots + (w.row < op.tokens ? w.row : w.row - op.tokens) * op.slots_token + e);
+            return __ldg(op.slots + (w.row >> 1) * op.slots_token + e);
         };
         Walk at(div, u0);
         int32_t slot = slot_of(at);
@@ -191,7 +200,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             const bool there = slot >= 0 && slot < op.pool_rows;
             if (!there && slot != kNotFound) bits |= ASU_ST_BAD_QUERY;
             const uint64_t from = reinterpret_cast<uint64_t>(op.pool) +
-                                  static_cast<uint64_t>(at.row < op.tokens ? at.row : at.row - op.tokens) * op.pool_token +
+                                  static_cast<uint64_t>(at.row >> 1) * op.pool_token +
                                   static_cast<uint64_t>(there ? slot : 0) * op.pool_pitch;
             const uint32_t valid = __ballot_sync(0xffffffffu, there);
             at.next(div);
@@ -251,11 +260,11 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             bool before_first = true;  // was tile n - 1 the first of its piece?
             for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
                 const bool first = at.u == u0 || at.tile == 0;
-                const bool half = at.row >= op.tokens;
+                const bool half = at.row & 1;
                 if (first) {
                     // the token before is finished first: its weights do not depend on this one's q
                     if (n > 0) output(n - 1, !before_first);
-                    wait(bar(kQuery), segment++);
+                    if (at.u == u0 || !half) wait(bar(kQuery), segment++);
                 }
                 if (n >= 1) wait(bar(kScoresRead), n - 1);
 #pragma unroll 1
@@ -355,10 +364,10 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         float m = -INFINITY;
         uint64_t l2 = 0;  // the sum of the even and of the odd entries
         Walk at(div, u0);
-        load_q(at.row < op.tokens ? at.row : at.row - op.tokens);
+        load_q(at.row >> 1);
         for (uint32_t n = 0; at.u < u1; at.next(div), ++n) {
-            const int half = at.row >= op.tokens;
-            const int64_t token = at.row - (half ? op.tokens : 0);
+            const int half = at.row & 1;
+            const int64_t token = at.row >> 1;
             const int tile = at.tile;
             const bool first = at.u == u0 || tile == 0;
             const bool last = at.u + 1 == u1 || tile + 1 == tiles;
@@ -366,10 +375,9 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 m = -INFINITY;
                 l2 = 0;
                 // the next token's q to L2: its loads come between two tokens, where nothing hides them
-                const int32_t next = (at.row + 1) * tiles;
+                const int32_t next = (token + 1) * 2 * tiles;
                 if (next < u1 && head < op.heads) {
-                    const __nv_bfloat16* q =
-                        op.q + (at.row + 1 < op.tokens ? at.row + 1 : at.row + 1 - op.tokens) * op.q_token + head * op.q_head;
+                    const __nv_bfloat16* q = op.q + (token + 1) * op.q_token + head * op.q_head;
 #pragma unroll
                     for (int k = 0; k < kDim; k += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k));
                 }
@@ -448,9 +456,9 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 for (int i = 0; i < 32; ++i) scratch.p[(to * 32 + i) * 128 + head] = p[i];
             }
             if (last) {
-                // this token's scores are all made: the next one's q, whose first scores then run
+                // a token's scores are all made: the next one's q, whose first scores then run
                 // beside what follows here
-                if (at.u + 1 < u1) load_q(at.row + 1 < op.tokens ? at.row + 1 : at.row + 1 - op.tokens);
+                if (at.u + 1 < u1 && half) load_q(token + 1);
                 float l, odd;
                 unpair(l2, l, odd);
                 l += odd;
@@ -468,13 +476,13 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                         tc::tmem_wait_load(o);
                         if (head < op.heads) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t w[4];
+                            for (int i = 0; i < 2; ++i) {
+                                uint32_t w[8];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    w[k] = pack_bf16(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                                     __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-                                reinterpret_cast<uint4*>(out + c)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                                for (int k = 0; k < 8; ++k)
+                                    w[k] = pack_bf16(__uint_as_float(o[16 * i + 2 * k]) * inv,
+                                                     __uint_as_float(o[16 * i + 2 * k + 1]) * inv);
+                                store32(out + c + 16 * i, w);
                             }
                         }
                         __syncwarp();
@@ -517,111 +525,162 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
     }
 }
 
+constexpr int kFinishTiles = 4;  // tiles whose weights one block sums
+
 // Joins the pieces of the rows that several CTAs share, and sums the weights over the heads.
-//   blocks y < 64: 8 output columns of one half of a token; a thread takes a head's 8 columns of every
-//                  kGroups-th piece, the groups are added up in shared memory in their order
-//   other blocks:  one tile's weights: weights_j = sum_h p_hj 2^(ref_h - lse_h)
+//   blocks y < kJoins: a thread takes some columns of a head, of one half of a token.  kGroups 1: 16 columns,
+//                  for rows of few pieces.  kGroups 8: 8 columns and every eighth piece; the groups are
+//                  added up in shared memory in their order
+//   other blocks:  weights_j = sum_h p_hj 2^(ref_h - lse_h) of kFinishTiles tiles, a warp two entries at a time
+// Loads that do not depend on one another are issued together: the blocks are short and wait for little else.
 template <int kGroups>
-__global__ void __launch_bounds__(128 * kGroups)
+__global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups)
 kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scratch) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_sum[kGroups][10][128];  // 8 columns, sum of exponentials, maximum
+    constexpr int kThreads = kGroups == 1 ? 256 : 128 * kGroups, kWarps = kThreads / 32;
+    constexpr int kCols = kGroups == 1 ? 16 : 8, kBlockCols = kGroups == 1 ? 32 : 8, kJoins = 512 / kBlockCols;
+    constexpr int kParts = kThreads / 128;  // of the pieces, where a block sums weights
+    __shared__ float s_shared[kGroups == 1 ? kFinishTiles * 128 : 10 * kGroups * 128];
     const int64_t token = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int head = tid & 127, group = tid >> 7;
-    const bool joins = blockIdx.y < 64;
-    const int half = joins ? blockIdx.y >> 5 : 0;
-    const int32_t first = (half * op.tokens + static_cast<int32_t>(token)) * div.tiles;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = tid & 127, group = tid >> 7;
+    const int y = blockIdx.y;
+    const int half = y < kJoins ? y / (kJoins / 2) : 0;  // the weights are of half 0's pieces
+    const int32_t first = (2 * static_cast<int32_t>(token) + half) * div.tiles;
     const int i0 = div.cta_of(first), i1 = div.cta_of(first + div.tiles - 1);
-    if (joins && i0 == i1) return;  // written by its one CTA
-    float m = -INFINITY, l = 0.0f;  // of the token's head, maximum in base 2
-    if (i0 != i1) {
-        for (int i = i0 + group; i <= i1; i += kGroups) m = fmaxf(m, scratch.ml[div.piece(i, first) * 256 + head]);
-        s_sum[group][9][head] = m;
-        __syncthreads();
+    // running maximum (base 2) and sum of this thread's pieces, two at a time
+    float m = -INFINITY, l = 0.0f;
+    auto join = [&](float m0, float l0, float m1, float l1, float& old, float& f0, float& f1) {
+        const float top = fmaxf(m, fmaxf(m0, m1));
+        old = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        f0 = m0 == -INFINITY ? 0.0f : exp2_fast(m0 - top);
+        f1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - top);
+        l = fmaf(l, old, fmaf(l0, f0, l1 * f1));
+        m = top;
+    };
+    auto load_ml = [&](int i, float& pm, float& pl) {
+        const float* ml = scratch.ml + div.piece(i, first) * 256 + head;
+        pm = i <= i1 ? __ldcg(ml) : -INFINITY;
+        pl = i <= i1 ? __ldcg(ml + 128) : 0.0f;
+    };
+    if (y < kJoins) {
+        if (i0 == i1) return;  // written by its one CTA
+        const int c0 = y % (kJoins / 2) * kBlockCols + (kGroups == 1 ? group * kCols : 0);
+        constexpr int kStep = kGroups;
+        float acc[kCols] = {};
+        for (int i = i0 + (kGroups == 1 ? 0 : group); i <= i1; i += 2 * kStep) {
+            float m0, l0, m1, l1, old, f0, f1, a[kCols], b[kCols];
+            load_ml(i, m0, l0);
+            load_ml(i + kStep, m1, l1);
+            const float* o0 = scratch.o + (static_cast<int64_t>(div.piece(i, first)) * 256 + c0) * 128 + head;
+            const float* o1 =
+                scratch.o + (static_cast<int64_t>(div.piece(i + kStep <= i1 ? i + kStep : i, first)) * 256 + c0) * 128 + head;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s_sum[g][9][head]);
-        float acc[8] = {};
-        const int c0 = (blockIdx.y & 31) * 8;
-#pragma unroll 2
-        for (int i = i0 + group; i <= i1; i += kGroups) {
-            const int piece = div.piece(i, first);
-            const float pm = scratch.ml[piece * 256 + head];
-            const float f = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
-            l += scratch.ml[piece * 256 + 128 + head] * f;
-            if (joins) {
-                const float* o = scratch.o + (static_cast<int64_t>(piece) * 256 + c0) * 128 + head;
+            for (int c = 0; c < kCols; ++c) {
+                a[c] = __ldcg(o0 + c * 128);
+                b[c] = __ldcg(o1 + c * 128);
+            }
+            join(m0, l0, m1, l1, old, f0, f1);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) acc[c] += o[c * 128] * f;
+            for (int c = 0; c < kCols; ++c) acc[c] = fmaf(acc[c], old, fmaf(a[c], f0, b[c] * f1));
+        }
+        if constexpr (kGroups > 1) {
+            float* mine = s_shared + group * 128 + head;  // [10][kGroups][128]
+            mine[8 * kGroups * 128] = m;
+            mine[9 * kGroups * 128] = l;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) mine[c * kGroups * 128] = acc[c];
+            __syncthreads();
+            if (group != 0) return;
+            float f[kGroups];
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) m = fmaxf(m, mine[(8 * kGroups + g) * 128]);
+            l = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const float mg = mine[(8 * kGroups + g) * 128];
+                f[g] = mg == -INFINITY ? 0.0f : exp2_fast(mg - m);
+                l = fmaf(mine[(9 * kGroups + g) * 128], f[g], l);
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                acc[c] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) acc[c] = fmaf(mine[(c * kGroups + g) * 128], f[g], acc[c]);
             }
         }
-        s_sum[group][8][head] = l;
+        if (head >= op.heads) return;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint32_t w[kCols / 2];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) s_sum[group][c][head] = acc[c];
+        for (int c = 0; c < kCols; c += 2) w[c / 2] = pack_bf16(acc[c] * inv, acc[c + 1] * inv);
+        __nv_bfloat16* out = op.out + (token * op.heads + head) * kLatent + half * 256 + c0;
+        if constexpr (kCols == 16) store32(out, w);
+        else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (y == 0 && c0 == 0)
+            op.lse[token * op.heads + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        return;
+    }
+    const int tile0 = (y - kJoins) * kFinishTiles, count = min(kFinishTiles, div.tiles - tile0);
+    constexpr int kBatch = 128 / kWarps < 8 ? 128 / kWarps : 8;
+    const uint32_t* from = scratch.p + (token * div.tiles + tile0) * 32 * 128 + lane * 4;
+    uint4 p[kBatch];  // row k: two entries, the halves of the words
+    auto load_rows = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = k0 + i * kWarps;
+            p[i] = k < count * 32 ? __ldcg(reinterpret_cast<const uint4*>(from + k * 128)) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    load_rows(warp);
+    float ref[kFinishTiles];
+#pragma unroll
+    for (int k = 0; k < kFinishTiles; ++k)
+        ref[k] = group == 0 && k < count ? __ldcg(scratch.ref + (token * div.tiles + tile0 + k) * 128 + head) : 0.0f;
+    if (i0 == i1) {
+        if (group == 0 && head < op.heads) m = op.lse[token * op.heads + head] * 1.4426950408889634f, l = 1.0f;
+    } else {  // the joining blocks may not have written lse yet
+        for (int i = i0 + group; i <= i1; i += 2 * kParts) {
+            float m0, l0, m1, l1, old, f0, f1;
+            load_ml(i, m0, l0);
+            load_ml(i + kParts, m1, l1);
+            join(m0, l0, m1, l1, old, f0, f1);
+        }
+        s_shared[tid] = m;
+        s_shared[kThreads + tid] = l;
         __syncthreads();
-        l = 0.0f;
+        if (group == 0) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) l += s_sum[g][8][head];
-        if (joins) {
-            if (group == 0 && head < op.heads) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                uint32_t w[4];
-#pragma unroll
-                for (int c = 0; c < 8; c += 2) {
-                    float a = 0.0f, b = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        a += s_sum[g][c][head];
-                        b += s_sum[g][c + 1][head];
-                    }
-                    w[c / 2] = pack_bf16(a * inv, b * inv);
-                }
-                *reinterpret_cast<uint4*>(op.out + (token * op.heads + head) * kLatent + half * 256 + c0) =
-                    make_uint4(w[0], w[1], w[2], w[3]);
-                if (blockIdx.y == 0)
-                    op.lse[token * op.heads + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            for (int g = 1; g < kParts; ++g) {
+                float old, f0, f1;
+                join(s_shared[g * 128 + head], s_shared[kThreads + g * 128 + head], -INFINITY, 0.0f, old, f0, f1);
             }
-            return;
         }
         __syncthreads();
     }
-    float* s_lse = s_sum[0][0];  // base 2
     if (group == 0) {
-        float v = -INFINITY;
-        if (head < op.heads) {
-            if (i0 != i1) v = l > 0.0f ? m + log2f(l) : -INFINITY;
-            else v = op.lse[token * op.heads + head] * 1.4426950408889634f;
-        }
-        s_lse[head] = v;
+        const float lse = l > 0.0f && head < op.heads ? m + log2f(l) : -INFINITY;  // base 2
+#pragma unroll
+        for (int k = 0; k < kFinishTiles; ++k) s_shared[k * 128 + head] = lse == -INFINITY ? 0.0f : exp2_fast(ref[k] - lse);
     }
     __syncthreads();
-    const int tile = blockIdx.y - 64;
-    const int64_t at = token * div.tiles + tile;
-    float f[4];
+    for (int k0 = warp; k0 < count * 32; k0 += kBatch * kWarps) {
+        if (k0 != warp) load_rows(k0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int h = lane * 4 + i;
-        f[i] = s_lse[h] == -INFINITY ? 0.0f : exp2_fast(scratch.ref[at * 128 + h] - s_lse[h]);
-    }
-#pragma unroll 4
-    for (int k = warp; k < 32; k += 4 * kGroups) {  // a warp a pair of entries
-        const uint4 p = *reinterpret_cast<const uint4*>(scratch.p + (at * 32 + k) * 128 + lane * 4);
-        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-        float a = 0.0f, b = 0.0f;
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = k0 + i * kWarps;
+            const float4 f = *reinterpret_cast<const float4*>(s_shared + k / 32 % kFinishTiles * 128 + lane * 4);
+            float a = __uint_as_float(p[i].x << 16) * f.x, b = __uint_as_float(p[i].x & 0xffff0000u) * f.x;
+            a = fmaf(__uint_as_float(p[i].y << 16), f.y, a), b = fmaf(__uint_as_float(p[i].y & 0xffff0000u), f.y, b);
+            a = fmaf(__uint_as_float(p[i].z << 16), f.z, a), b = fmaf(__uint_as_float(p[i].z & 0xffff0000u), f.z, b);
+            a = fmaf(__uint_as_float(p[i].w << 16), f.w, a), b = fmaf(__uint_as_float(p[i].w & 0xffff0000u), f.w, b);
+            // the lower lanes go on with the first entry, the upper ones with the second
+            float sum = (lane < 16 ? a : b) + __shfl_xor_sync(0xffffffffu, lane < 16 ? b : a, 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a = fmaf(__uint_as_float(w[i] << 16), f[i], a);
-            b = fmaf(__uint_as_float(w[i] & 0xffff0000u), f[i], b);
+            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int e = tile0 * kTile + 2 * k + (lane >> 4);
+            if ((lane & 15) == 0 && k < count * 32 && e < op.topk) op.weights[token * op.topk + e] = __float2bfloat16(sum);
         }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, d);
-            b += __shfl_xor_sync(0xffffffffu, b, d);
-        }
-        const int e = tile * kTile + 2 * k;
-        if (lane == 0 && e < op.topk) op.weights[token * op.topk + e] = __float2bfloat16(a);
-        if (lane == 1 && e + 1 < op.topk) op.weights[token * op.topk + e + 1] = __float2bfloat16(b);
     }
 }
 
@@ -662,9 +721,11 @@ int launch_wide(cudaStream_t s, const Operands& op, void* workspace) {
     for (int i = 1; i < d.ctas && most < 3; ++i)
         if (d.start(i) % d.tiles != 0) most = d.start(i + 1) / d.tiles == d.start(i) / d.tiles && i + 1 < d.ctas ? 3 : 2;
     if (rc != ASU_OK || (most == 1 && op.weights == nullptr)) return rc;
-    const dim3 grid(static_cast<unsigned>(op.tokens), 64 + (op.weights != nullptr ? d.tiles : 0));
-    if (most > 2) return launch_pdl(kv4_finish_wide_kernel<8>, grid, dim3(1024), 0, s, op, d, scratch);
-    return launch_pdl(kv4_finish_wide_kernel<2>, grid, dim3(256), 0, s, op, d, scratch);
+    const int sums = op.weights != nullptr ? (d.tiles + kFinishTiles - 1) / kFinishTiles : 0;
+    const unsigned tokens = static_cast<unsigned>(op.tokens);
+    if (most > 2)
+        return launch_pdl(kv4_finish_wide_kernel<8>, dim3(tokens, 64 + sums), dim3(1024), 0, s, op, d, scratch);
+    return launch_pdl(kv4_finish_wide_kernel<1>, dim3(tokens, 16 + sums), dim3(256), 0, s, op, d, scratch);
 }
 
 }  // namespace kv4

@@ -431,9 +431,11 @@ int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows, uint64_t p
  * with k_j all 576 values and v_j the first 512.  q: bf16, strides in elements; out [tokens, heads,
  * 512] bf16; lse [tokens, heads] fp32; weights [tokens, topk] bf16 (nullable).  A token without any
  * entry gets out 0, lse -inf and weights 0.  Any other slot outside [0, pool_rows) counts as not
- * there and sets ASU_ST_BAD_QUERY in status[0] (nullable).  `workspace`: device memory of
- * asu_kv4_attention_workspace_bytes(...) bytes on the current device, 16-byte aligned, used by this
- * call alone until it is done (-1: sizes out of range).  Results do not depend on scheduling.
+ * there and sets ASU_ST_BAD_QUERY in status[0] (nullable); ASU_ST_TIMEOUT there means that the kernel
+ * gave up waiting for itself and that the outputs are not valid.  pool and its strides are 16-byte
+ * aligned, out 32.  `workspace`: device memory of asu_kv4_attention_workspace_bytes(...) bytes on
+ * the current device, 32-byte aligned, used by this call alone until it is done (-1: sizes out of
+ * range).  Results do not depend on scheduling.
  * Limits: heads <= 128, tokens <= 65535, topk <= 16384. */
 int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights);
 int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* pool,
