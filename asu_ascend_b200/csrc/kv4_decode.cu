@@ -52,7 +52,7 @@ enum Bar {
     kOutput,    // all of them: the rest of the rows and the weights are free
     kScores,    // the tile's scores are made
     kWeights,   // its weights are in shared memory and the scores read (128 threads)
-    kQuery,     // the row of work's q is in place (128 threads)
+    kQuery,     // the token's q is in place (128 threads)
     kDrain,
     kBars
 };
@@ -71,8 +71,8 @@ struct Layout {
 struct Scratch {
     float* ml;         // [2 * ctas][2][kN] reference (base 2) and sum of a piece
     float* o;          // [2 * ctas][kN][512] its output
-    float* ref;        // [rows of work][tiles][kN] the reference of a tile's weights
-    __nv_bfloat16* p;  // [rows of work][tiles][128][kN] a tile's weights
+    float* ref;        // [tokens][tiles][kN] the reference of a tile's weights
+    __nv_bfloat16* p;  // [tokens][tiles][128][kN] a tile's weights
 };
 
 // What a slot that is not there reads: a row of zeros.
@@ -163,9 +163,8 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         uint32_t low_scales[4], high_scales[4];
         int32_t slot[4];
         Walk ahead(div, u0);
-        int token = ahead.row % op.tokens;
         auto load_slots = [&] {
-            const int32_t* row = op.slots + token * op.slots_token;
+            const int32_t* row = op.slots + ahead.row * op.slots_token;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int e = ahead.tile * kTile + i * 32 + row0;
@@ -173,7 +172,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
             }
         };
         auto load_rows = [&] {
-            const uint8_t* pool = op.pool + static_cast<uint64_t>(token) * op.pool_token;
+            const uint8_t* pool = op.pool + static_cast<uint64_t>(ahead.row) * op.pool_token;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool there = slot[i] >= 0 && slot[i] < op.pool_rows;
@@ -187,14 +186,9 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 high_scales[i] = load2(p + kScaleOffset + 16 + chunk * 2);
             }
         };
-        auto next = [&] {
-            const int row = ahead.row;
-            ahead.next(div);
-            if (ahead.row != row && ++token == op.tokens) token = 0;
-        };
         load_slots();
         load_rows();
-        next();
+        ahead.next(div);
         load_slots();
         const uint32_t at = base + L::kRows + quarter * kBlock + row0 * 128 + (((lp * 4) ^ (row0 & 7)) << 4);
         const uint32_t rope_at = base + L::kRope + row0 * 128 + ((rope_chunk ^ (row0 & 7)) << 4);
@@ -216,7 +210,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(bar(kFullHigh));
             load_rows();
-            next();
+            ahead.next(div);
             load_slots();
         }
         if (bits) flag_status(op.status, 0, bits);
@@ -269,14 +263,13 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         // ---- softmax: a thread an entry of the tile; for the output, a thread a latent of 128 ----
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         auto softmax_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // these four warps
-        auto load_q = [&](int row) {
-            const int token = row % op.tokens, head0 = row / op.tokens * kN;
+        auto load_q = [&](int token) {
             const __nv_bfloat16* q = op.q + token * op.q_token + (tid & 7) * 8;
             const uint32_t to0 = base + L::kQ + (((tid ^ (tid >> 3)) & 7) << 4);
 #pragma unroll 1
             for (int h = tid >> 3; h < kN; h += 16) {
-                const bool there = head0 + h < op.heads;
-                const __nv_bfloat16* from = q + (there ? head0 + h : 0) * op.q_head;
+                const bool there = h < op.heads;
+                const __nv_bfloat16* from = q + (there ? h : 0) * op.q_head;
                 if (op.q_aligned || !there) {
 #pragma unroll
                     for (int k = 0; k < 9; ++k)
@@ -299,16 +292,15 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         float l[kN];                           // this thread's entries' weights by head
         Walk at(div, u0);
         load_q(at.row);
-        int token = at.row % op.tokens;
-        auto slot_here = [&](const Walk& w, int tok) -> bool {
+        auto slot_here = [&](const Walk& w) -> bool {
             const int e = w.tile * kTile + tid;
             if (w.u >= u1 || e >= op.topk) return false;
-            const int32_t s = __ldg(op.slots + tok * op.slots_token + e);
+            const int32_t s = __ldg(op.slots + w.row * op.slots_token + e);
             return s >= 0 && s < op.pool_rows;
         };
-        bool there = slot_here(at, token);
+        bool there = slot_here(at);
         for (uint32_t n = 0; at.u < u1; ++n) {
-            const int row = at.row, tile = at.tile;
+            const int token = at.row, tile = at.tile;
             const bool first = at.u == u0 || tile == 0;
             const bool last = at.u + 1 == u1 || tile + 1 == tiles;
             if (first) {
@@ -374,7 +366,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                     tc::tmem_wait_store();
                 }
             }
-            const int64_t unit = static_cast<int64_t>(row) * tiles + tile;
+            const int64_t unit = static_cast<int64_t>(token) * tiles + tile;
             if (op.weights != nullptr && tid < kN) scratch.ref[unit * kN + tid] = -s_minus_ref[tid];
 #pragma unroll
             for (int c0 = 0; c0 < kN; c0 += kC) {
@@ -406,11 +398,9 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
             tc::fence_before();
             tc::mbar_arrive(bar(kWeights));
             at.next(div);
-            const int was = token;
-            if (at.row != row && ++token == op.tokens) token = 0;
-            there = slot_here(at, token);
+            there = slot_here(at);
             if (last) {
-                // this row's scores are all made: the next one's q comes beside the output products
+                // this token's scores are all made: the next one's q comes beside the output products
                 if (at.u < u1) load_q(at.row);
                 // sums over the entries: within the warps, then the four
 #pragma unroll
@@ -421,8 +411,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                     if (lane == (h & 31)) s_top[warp][h] = __float_as_int(x);
                 }
                 softmax_sync();
-                const int head0 = row / op.tokens * kN;
-                const int row_start = row * tiles;
+                const int row_start = token * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
                 const int piece = div.piece(blockIdx.x, row_start);
                 if (tid < kN) {
@@ -430,8 +419,8 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                                       (__int_as_float(s_top[2][tid]) + __int_as_float(s_top[3][tid]));
                     if (whole) {
                         s_fade[tid] = sum > 0.0f ? 1.0f / sum : 0.0f;
-                        if (head0 + tid < op.heads)
-                            op.lse[static_cast<int64_t>(was) * op.heads + head0 + tid] =
+                        if (tid < op.heads)
+                            op.lse[static_cast<int64_t>(token) * op.heads + tid] =
                                 sum > 0.0f ? (log2f(sum) - s_minus_ref[tid]) * 0.6931471805599453f : -INFINITY;
                     } else {
                         scratch.ml[piece * 2 * kN + tid] = sum > 0.0f ? -s_minus_ref[tid] : -INFINITY;
@@ -448,10 +437,10 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                     tc::tmem_wait_load(o);
                     const int latent = c0 / kN * 128 + tid, h0 = c0 % kN;
                     if (whole) {
-                        __nv_bfloat16* to = op.out + (static_cast<int64_t>(was) * op.heads + head0 + h0) * kLatent + latent;
+                        __nv_bfloat16* to = op.out + (static_cast<int64_t>(token) * op.heads + h0) * kLatent + latent;
 #pragma unroll
                         for (int h = 0; h < kC; ++h)
-                            if (head0 + h0 + h < op.heads)
+                            if (h0 + h < op.heads)
                                 to[h * kLatent] = __float2bfloat16(__uint_as_float(o[h]) * s_fade[h0 + h]);
                     } else {
                         float* to = scratch.o + (static_cast<int64_t>(piece) * kN + h0) * kLatent + latent;
@@ -480,47 +469,65 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     }
 }
 
-// Joins the pieces of rows that several CTAs share, and sums the weights over the heads.
-//   blocks y < heads: one head of a token, 4 latents a thread
-//   other blocks:     one tile, an entry a thread: weights_j = sum_h p_hj 2^(ref_h - lse_h)
+// Joins the pieces of tokens that several CTAs share, and sums the weights over the heads.
+//   blocks y < joins: two heads of a token, 4 latents a thread
+//   other blocks:     two tiles, an entry a thread: weights_j = sum_h p_hj 2^(ref_h - lse_h)
+// Loads that do not depend on one another are issued together: the blocks are short and wait for little else.
 template <int kN>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_factor[ASU_KV4_MAX_HEADS];
-    const int token = blockIdx.x, tid = threadIdx.x;
-    // reference and sum (base 2) of a head over its pieces; the CTAs of its row
-    auto total = [&](int head, int& i0, int& i1, float& m, float& l) {
-        const int first = (head / kN * op.tokens + token) * div.tiles;
-        i0 = div.cta_of(first);
-        i1 = div.cta_of(first + div.tiles - 1);
-        if (i0 == i1) return;
-        m = -INFINITY, l = 0.0f;
-#pragma unroll 4
-        for (int i = i0; i <= i1; ++i) m = fmaxf(m, scratch.ml[div.piece(i, first) * 2 * kN + head % kN]);
-#pragma unroll 4
-        for (int i = i0; i <= i1; ++i) {
-            const float* ml = scratch.ml + div.piece(i, first) * 2 * kN + head % kN;
-            l += ml[kN] * (ml[0] == -INFINITY ? 0.0f : exp2_fast(ml[0] - m));
+    __shared__ float s_factor[2][kN];
+    const int token = blockIdx.x, joins = (op.heads + 1) / 2;
+    const int tid = threadIdx.x & 127, part = threadIdx.x >> 7;
+    const int first = token * div.tiles;
+    const int i0 = div.cta_of(first), i1 = div.cta_of(first + div.tiles - 1);
+    constexpr int kBatch = 4;  // pieces at a time
+    // running reference (base 2) and sum of a head; factors of what is there and of the next pieces
+    float m = -INFINITY, l = 0.0f, old, f[kBatch];
+    float pm[kBatch], pl[kBatch];
+    auto load_ml = [&](int i, int head) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const bool here = i + k <= i1;
+            const float* ml = scratch.ml + div.piece(here ? i + k : i, first) * 2 * kN + head;
+            pm[k] = here ? __ldcg(ml) : -INFINITY;
+            pl[k] = __ldcg(ml + kN);
         }
     };
-    if (static_cast<int>(blockIdx.y) < op.heads) {
-        const int head = blockIdx.y;
-        int i0, i1;
-        float m, l;
-        total(head, i0, i1, m, l);
-        if (i0 == i1) return;  // written by its one CTA
-        const int first = (head / kN * op.tokens + token) * div.tiles;
+    auto join = [&] {
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = fmaxf(top, pm[k]);
+        old = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        l *= old;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            f[k] = pm[k] == -INFINITY ? 0.0f : exp2_fast(pm[k] - top);
+            l = fmaf(pl[k], f[k], l);
+        }
+        m = top;
+    };
+    if (static_cast<int>(blockIdx.y) < joins) {
+        const int head = 2 * blockIdx.y + part;
+        if (i0 == i1 || head >= op.heads) return;  // written by its one CTA
         float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int i = i0; i <= i1; ++i) {
-            const int piece = div.piece(i, first);
-            const float pm = scratch.ml[piece * 2 * kN + head % kN];
-            const float f = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
-            const float4 v =
-                reinterpret_cast<const float4*>(scratch.o + (static_cast<int64_t>(piece) * kN + head % kN) * kLatent)[tid];
-            acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+        for (int i = i0; i <= i1; i += kBatch) {
+            load_ml(i, head);
+            float4 v[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+                v[k] = i + k <= i1 ? __ldcg(reinterpret_cast<const float4*>(
+                                                scratch.o + (static_cast<int64_t>(div.piece(i + k, first)) * kN + head) * kLatent) + tid)
+                                   : make_float4(0, 0, 0, 0);
+            join();
+            acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                acc.x = fmaf(v[k].x, f[k], acc.x), acc.y = fmaf(v[k].y, f[k], acc.y);
+                acc.z = fmaf(v[k].z, f[k], acc.z), acc.w = fmaf(v[k].w, f[k], acc.w);
+            }
         }
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         reinterpret_cast<uint2*>(op.out + (static_cast<int64_t>(token) * op.heads + head) * kLatent)[tid] =
@@ -530,37 +537,40 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
                 l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
         return;
     }
-    const int tile = blockIdx.y - op.heads;
-    const int parts = (op.heads + kN - 1) / kN;
-    for (int head = tid; head < parts * kN; head += 128) {  // the joining blocks may not have written lse yet
-        float f = 0.0f;
-        if (head < op.heads) {
-            int i0, i1;
-            float m, l;
-            total(head, i0, i1, m, l);
-            const float lse = i0 == i1 ? op.lse[static_cast<int64_t>(token) * op.heads + head] * 1.4426950408889634f
-                                       : (l > 0.0f ? m + log2f(l) : -INFINITY);
-            const int64_t unit = static_cast<int64_t>(head / kN * op.tokens + token) * div.tiles + tile;
-            if (lse != -INFINITY) f = exp2_fast(scratch.ref[unit * kN + head % kN] - lse);
+    const int tile = 2 * (blockIdx.y - joins) + part;
+    const bool here = tile < div.tiles;
+    const int64_t unit = static_cast<int64_t>(token) * div.tiles + (here ? tile : 0);
+    const uint4* p = reinterpret_cast<const uint4*>(scratch.p + (unit * kTile + tid) * kN);
+    uint4 v[kN / 8];
+#pragma unroll
+    for (int i = 0; i < kN / 8; ++i) v[i] = __ldcg(p + i);
+    if (tid < kN) {
+        const float ref = __ldcg(scratch.ref + unit * kN + tid);
+        float lse = -INFINITY;  // base 2; the joining blocks may not have written it yet
+        if (tid < op.heads) {
+            if (i0 == i1) {
+                lse = op.lse[static_cast<int64_t>(token) * op.heads + tid] * 1.4426950408889634f;
+            } else {
+                for (int i = i0; i <= i1; i += kBatch) {
+                    load_ml(i, tid);
+                    join();
+                }
+                if (l > 0.0f) lse = m + log2f(l);
+            }
         }
-        s_factor[head] = f;
+        s_factor[part][tid] = lse == -INFINITY ? 0.0f : exp2_fast(ref - lse);
     }
     __syncthreads();
     const int e = tile * kTile + tid;
-    if (e >= op.topk) return;
+    if (!here || e >= op.topk) return;
     float w = 0.0f;
-    for (int part = 0; part < parts; ++part) {
-        const int64_t unit = static_cast<int64_t>(part * op.tokens + token) * div.tiles + tile;
-        const uint4* p = reinterpret_cast<const uint4*>(scratch.p + (unit * kTile + tid) * kN);
 #pragma unroll
-        for (int i = 0; i < kN / 8; ++i) {
-            const uint4 v = __ldg(p + i);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < kN / 8; ++i) {
+        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                w = fmaf(__uint_as_float(x[k] << 16), s_factor[part * kN + i * 8 + 2 * k], w);
-                w = fmaf(__uint_as_float(x[k] & 0xffff0000u), s_factor[part * kN + i * 8 + 2 * k + 1], w);
-            }
+        for (int k = 0; k < 4; ++k) {
+            w = fmaf(__uint_as_float(x[k] << 16), s_factor[part][i * 8 + 2 * k], w);
+            w = fmaf(__uint_as_float(x[k] & 0xffff0000u), s_factor[part][i * 8 + 2 * k + 1], w);
         }
     }
     op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(w);
@@ -568,9 +578,8 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
 
 int columns_of(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
-Division division(int64_t tokens, int64_t heads, int64_t topk, int sms) {
-    const int n = columns_of(heads);
-    return Division((heads + n - 1) / n * tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms);
+Division division(int64_t tokens, int64_t topk, int sms) {
+    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms);  // no entry: one empty tile
 }
 
 void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
@@ -584,7 +593,7 @@ void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
 
 template <int kN>
 int launch(cudaStream_t s, const Operands& op, void* workspace) {
-    const Division d = division(op.tokens, op.heads, op.topk, asu_sm_count());
+    const Division d = division(op.tokens, op.topk, asu_sm_count());
     int64_t at[5];
     layout(d, kN, op.weights != nullptr, at);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -600,15 +609,15 @@ int launch(cudaStream_t s, const Operands& op, void* workspace) {
     if (rc != ASU_OK || (!shared_rows && op.weights == nullptr)) return rc;
     return launch_pdl(kv4_finish_kernel<kN>,
                       dim3(static_cast<unsigned>(op.tokens),
-                           static_cast<unsigned>(op.heads + (op.weights != nullptr ? d.tiles : 0))),
-                      dim3(128), 0, s, op, d, scratch);
+                           static_cast<unsigned>((op.heads + 1) / 2 + (op.weights != nullptr ? (d.tiles + 1) / 2 : 0))),
+                      dim3(256), 0, s, op, d, scratch);
 }
 
 }  // namespace
 
 int64_t tall_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
     int64_t at[5];
-    layout(division(tokens, heads, topk, asu_sm_count()), columns_of(heads), weights, at);
+    layout(division(tokens, topk, asu_sm_count()), columns_of(heads), weights, at);
     return at[4];
 }
 
