@@ -115,7 +115,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     __shared__ int s_dead;
     __shared__ float s_minus_ref[kN];  // minus the reference, base 2; +inf while there is none
     __shared__ float s_fade[kN];       // what a new reference multiplies sums and output by; later 1 / sum
-    __shared__ int s_top[4][kN];       // each softmax warp's maximum, or sum
+    __shared__ __align__(8) int s_top[4][kN];       // each softmax warp's maximum, or sum
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
     auto bar = [&](int which) { return base + L::kBarsAt + 8u * which; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -402,14 +402,22 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
             if (last) {
                 // this token's scores are all made: the next one's q comes beside the output products
                 if (at.u < u1) load_q(at.row);
-                // sums over the entries: within the warps, then the four
+                // Sums over the entries: within the warps, then the four.  In each step a lane passes half of its
+                // heads on and adds the partner's to the other half.
 #pragma unroll
-                for (int h = 0; h < kN; ++h) {
-                    float x = l[h];
+                for (int d = 16, count = kN / 2; d > 0; d >>= 1, count >>= 1) {
+                    const bool upper = (lane & d) != 0;
+                    if (count == 0) l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
 #pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-                    if (lane == (h & 31)) s_top[warp][h] = __float_as_int(x);
+                    for (int h = 0; h < count; ++h) {
+                        const float other = __shfl_xor_sync(0xffffffffu, upper ? l[h] : l[h + count], d);
+                        l[h] = (upper ? l[h + count] : l[h]) + other;
+                    }
                 }
+                if constexpr (kN == 16) s_top[warp][lane / 2] = __float_as_int(l[0]);
+                if constexpr (kN == 32) s_top[warp][lane] = __float_as_int(l[0]);
+                if constexpr (kN == 64)
+                    *reinterpret_cast<int2*>(&s_top[warp][2 * lane]) = make_int2(__float_as_int(l[0]), __float_as_int(l[1]));
                 softmax_sync();
                 const int row_start = token * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
