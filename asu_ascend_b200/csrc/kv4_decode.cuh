@@ -106,26 +106,6 @@ __device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Pairs of floats in one register pair: one instruction for two.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // kv4_decode.cu: up to kTallHeads heads
