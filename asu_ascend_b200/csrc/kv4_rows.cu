@@ -10,9 +10,11 @@
 // corrected by one residual step (Markstein 1990), which gives every quotient that is representable
 // exactly -- the ties are.
 //
-// One warp per row, one lane per group: the lane loads its 32 bytes, needs no exchange with other
-// lanes for the maximum, and stores 8 bytes of nibbles and one scale byte; 8 lanes move the
-// rope part.  Bound by HBM: 1152 bytes in and 416 out per row (the other way round when reading).
+// A warp takes two rows at a time.  Writing, a lane has a group: it loads its 32 bytes, needs no exchange with
+// other lanes for the maximum, and stores 8 bytes of nibbles and one scale byte; 8 lanes move the rope part.
+// Reading, a lane has two words 32 apart, so that every store of the warp is of consecutive bytes.
+// 65536 rows (1152 bytes here, 416 there): 27 us to write, 3.8 TB/s, held up by instructions and latency together
+// (one row at a time 30 us, four 35); 20 us to read, 5.0 TB/s.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -24,7 +26,7 @@ using namespace kv4;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPackRows = 2, kUnpackRows = 4;  // a warp's rows at a time, their loads together
+constexpr int kRows = 2;  // a warp's rows at a time, their loads together
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
@@ -79,12 +81,12 @@ kv4_pack_kernel(const uint16_t* __restrict__ src, int64_t src_pitch, int64_t n, 
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     int32_t bits = 0;
-    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPackRows; i0 < n;
-         i0 += static_cast<int64_t>(gridDim.x) * kWarps * kPackRows) {
-        int64_t slot[kPackRows];
-        uint4 raw[kPackRows][2], rope[kPackRows];
+    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kRows; i0 < n;
+         i0 += static_cast<int64_t>(gridDim.x) * kWarps * kRows) {
+        int64_t slot[kRows];
+        uint4 raw[kRows][2], rope[kRows];
 #pragma unroll
-        for (int m = 0; m < kPackRows; ++m) {
+        for (int m = 0; m < kRows; ++m) {
             const int64_t i = i0 + m < n ? i0 + m : i0;
             slot[m] = i0 + m >= n ? kNotFound : slots != nullptr ? static_cast<int64_t>(__ldg(slots + i)) : i;
             const uint16_t* row = src + i * src_pitch;
@@ -92,7 +94,7 @@ kv4_pack_kernel(const uint16_t* __restrict__ src, int64_t src_pitch, int64_t n, 
             rope[m] = lane < kRope / 8 ? load8<kAlign>(row + kLatent + lane * 8) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int m = 0; m < kPackRows; ++m) {
+        for (int m = 0; m < kRows; ++m) {
             if (slot[m] == kNotFound) continue;
             if (slot[m] < 0 || slot[m] >= pool_rows) {
                 bits |= ASU_ST_BAD_QUERY;
@@ -166,13 +168,13 @@ kv4_unpack_kernel(const uint8_t* __restrict__ pool, int64_t pool_rows, uint64_t 
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     int32_t bits = 0;
-    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kUnpackRows; i0 < n;
-         i0 += static_cast<int64_t>(gridDim.x) * kWarps * kUnpackRows) {
-        uint32_t w[kUnpackRows][2], byte[kUnpackRows][2];
-        uint4 rope[kUnpackRows];
+    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kRows; i0 < n;
+         i0 += static_cast<int64_t>(gridDim.x) * kWarps * kRows) {
+        uint32_t w[kRows][2], byte[kRows][2];
+        uint4 rope[kRows];
         uint32_t there = 0;
 #pragma unroll
-        for (int m = 0; m < kUnpackRows; ++m) {
+        for (int m = 0; m < kRows; ++m) {
             const int64_t i = i0 + m;
             const int64_t slot = i >= n ? kNotFound : slots != nullptr ? static_cast<int64_t>(__ldg(slots + i)) : i;
             if (slot >= 0 && slot < pool_rows) {
@@ -189,7 +191,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ pool, int64_t pool_rows, uint64_t 
             }
         }
 #pragma unroll
-        for (int m = 0; m < kUnpackRows; ++m) {
+        for (int m = 0; m < kRows; ++m) {
             if (i0 + m >= n) break;
             uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
             if ((there >> m) & 1u) {
@@ -211,8 +213,8 @@ kv4_unpack_kernel(const uint8_t* __restrict__ pool, int64_t pool_rows, uint64_t 
     if (bits) flag_status(status, 0, bits);
 }
 
-dim3 grid_for(int64_t n, int rows) {
-    const int64_t blocks = (n + kWarps * rows - 1) / (kWarps * rows);
+dim3 grid_for(int64_t n) {
+    const int64_t blocks = (n + kWarps * kRows - 1) / (kWarps * kRows);
     return dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)));
 }
 
@@ -238,7 +240,7 @@ extern "C" int asu_kv4_pack(void* stream, const void* src, int32_t src_dtype, in
     const uint16_t* p = static_cast<const uint16_t*>(src);
     uint8_t* d = static_cast<uint8_t*>(pool);
     auto run = [&](auto kernel) {
-        return launch_pdl(kernel, grid_for(n, kPackRows), dim3(kThreads), 0, s, p, src_pitch, n, slots, d, pool_rows, pool_pitch,
+        return launch_pdl(kernel, grid_for(n), dim3(kThreads), 0, s, p, src_pitch, n, slots, d, pool_rows, pool_pitch,
                           status);
     };
     // 32-byte loads for rows that allow them, 16-byte ones, or single values
@@ -260,7 +262,7 @@ extern "C" int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows,
         return ASU_ERR_ARG;
     if (!pool_ok(pool, pool_rows, pool_pitch) || reinterpret_cast<uintptr_t>(dst) % 16 != 0 || dst_pitch % 8 != 0)
         return ASU_ERR_ALIGN;
-    return launch_pdl(kv4_unpack_kernel, grid_for(n, kUnpackRows), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
+    return launch_pdl(kv4_unpack_kernel, grid_for(n), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
                       static_cast<const uint8_t*>(pool), pool_rows, pool_pitch, slots, n,
                       static_cast<uint16_t*>(dst), dst_pitch, status);
 }
