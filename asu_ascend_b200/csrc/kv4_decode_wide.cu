@@ -68,8 +68,8 @@ enum Bar {
 };
 
 struct Scratch {
-    float* ml;         // [2 * ctas][2][128] running maximum (base 2) and sum of a piece
-    float* o;          // [2 * ctas][256][128] its output, columns by heads
+    float* ml;         // [2 * pairs][2 halves][2][128] running maximum (base 2) and sum of a piece
+    float* o;          // [2 * pairs][2 halves][256][128] its output, columns by heads
     float* ref;        // [tokens][tiles][128] the maximum that a tile's weights are relative to
     uint32_t* p;       // [tokens][tiles][32][128] a tile's weights, pairs of entries
 };
@@ -133,7 +133,8 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
     if (tid == 0 && s_tmem != 0) *dead = 1;
     pdl_wait();
 
-    const int32_t u0 = div.start(blockIdx.x), u1 = div.start(blockIdx.x + 1);
+    const int half = blockIdx.x & 1;  // of the output columns
+    const int32_t u0 = div.start(blockIdx.x >> 1), u1 = div.start((blockIdx.x >> 1) + 1);
     const int tiles = div.tiles;
 
     if (warp >= 4 && warp < 12) {
@@ -151,7 +152,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         uint32_t n = 0;
         for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
             const uint32_t raw = raw_at + (n & 1) * kRawTile;
-            const uint32_t mine = at.row & 1 ? 8 : 0, other = 8 - mine;  // chunks before this half's
+            const uint32_t mine = half ? 8 : 0, other = 8 - mine;  // chunks before this half's
             warp_wait(bar2(kRowsHere, n), n >> 1);
             if (n >= 1) warp_wait(bar(kFreeA), n - 1);
 #pragma unroll
@@ -190,7 +191,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         auto slot_of = [&](const Walk& w) -> int32_t {
             const int e = w.tile * kTile + row0 + lane;
             if (w.u >= u1 || e >= op.topk) return kNotFound;
-            return __ldg(op.slots + (w.row >> 1) * op.slots_token + e);
+            return __ldg(op.slots + w.row * op.slots_token + e);
         };
         Walk at(div, u0);
         int32_t slot = slot_of(at);
@@ -200,7 +201,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             const bool there = slot >= 0 && slot < op.pool_rows;
             if (!there && slot != kNotFound) bits |= ASU_ST_BAD_QUERY;
             const uint64_t from = reinterpret_cast<uint64_t>(op.pool) +
-                                  static_cast<uint64_t>(at.row >> 1) * op.pool_token +
+                                  static_cast<uint64_t>(at.row) * op.pool_token +
                                   static_cast<uint64_t>(there ? slot : 0) * op.pool_pitch;
             const uint32_t valid = __ballot_sync(0xffffffffu, there);
             at.next(div);
@@ -260,11 +261,10 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             bool before_first = true;  // was tile n - 1 the first of its piece?
             for (Walk at(div, u0); at.u < u1; at.next(div), ++n) {
                 const bool first = at.u == u0 || at.tile == 0;
-                const bool half = at.row & 1;
                 if (first) {
                     // the token before is finished first: its weights do not depend on this one's q
                     if (n > 0) output(n - 1, !before_first);
-                    if (at.u == u0 || !half) wait(bar(kQuery), segment++);
+                    wait(bar(kQuery), segment++);
                 }
                 if (n >= 1) wait(bar(kScoresRead), n - 1);
 #pragma unroll 1
@@ -278,7 +278,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                         for (int k = 0; k < 4; ++k)  // rope; the tile's first product overwrites
                             tc::mma_ts<kHigh>(kColS, kColQ + 4 * 32 + 8 * k, rows + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
                     }
-                    if (half == (part == 0)) low(rows);
+                    if ((half != 0) == (part == 0)) low(rows);
                     else high(rows);
                     tc::commit(part ? bar(kScores) : bar(kFreeA));
                 }
@@ -364,10 +364,9 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         float m = -INFINITY;
         uint64_t l2 = 0;  // the sum of the even and of the odd entries
         Walk at(div, u0);
-        load_q(at.row >> 1);
+        load_q(at.row);
         for (uint32_t n = 0; at.u < u1; at.next(div), ++n) {
-            const int half = at.row & 1;
-            const int64_t token = at.row >> 1;
+            const int64_t token = at.row;
             const int tile = at.tile;
             const bool first = at.u == u0 || tile == 0;
             const bool last = at.u + 1 == u1 || tile + 1 == tiles;
@@ -375,7 +374,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 m = -INFINITY;
                 l2 = 0;
                 // the next token's q to L2: its loads come between two tokens, where nothing hides them
-                const int32_t next = (token + 1) * 2 * tiles;
+                const int32_t next = (at.row + 1) * tiles;
                 if (next < u1 && head < op.heads) {
                     const __nv_bfloat16* q = op.q + (token + 1) * op.q_token + head * op.q_head;
 #pragma unroll
@@ -458,7 +457,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             if (last) {
                 // a token's scores are all made: the next one's q, whose first scores then run
                 // beside what follows here
-                if (at.u + 1 < u1 && half) load_q(token + 1);
+                if (at.u + 1 < u1) load_q(token + 1);
                 float l, odd;
                 unpair(l2, l, odd);
                 l += odd;
@@ -491,7 +490,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                         op.lse[token * op.heads + head] =
                             l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
                 } else {
-                    const int piece = div.piece(blockIdx.x, row_start);
+                    const int piece = div.piece(blockIdx.x >> 1, row_start) * 2 + half;
                     float* to = scratch.o + static_cast<int64_t>(piece) * 256 * 128 + head;
 #pragma unroll 1
                     for (int c = 0; c < 256; c += 32) {
@@ -546,7 +545,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = tid & 127, group = tid >> 7;
     const int y = blockIdx.y;
     const int half = y < kJoins ? y / (kJoins / 2) : 0;  // the weights are of half 0's pieces
-    const int32_t first = (2 * static_cast<int32_t>(token) + half) * div.tiles;
+    const int32_t first = static_cast<int32_t>(token) * div.tiles;
     const int i0 = div.cta_of(first), i1 = div.cta_of(first + div.tiles - 1);
     // running maximum (base 2) and sum of this thread's pieces, two at a time
     float m = -INFINITY, l = 0.0f;
@@ -559,7 +558,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
         m = top;
     };
     auto load_ml = [&](int i, float& pm, float& pl) {
-        const float* ml = scratch.ml + div.piece(i, first) * 256 + head;
+        const float* ml = scratch.ml + (div.piece(i, first) * 2 + half) * 256 + head;
         pm = i <= i1 ? __ldcg(ml) : -INFINITY;
         pl = i <= i1 ? __ldcg(ml + 128) : 0.0f;
     };
@@ -572,9 +571,9 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
             float m0, l0, m1, l1, old, f0, f1, a[kCols], b[kCols];
             load_ml(i, m0, l0);
             load_ml(i + kStep, m1, l1);
-            const float* o0 = scratch.o + (static_cast<int64_t>(div.piece(i, first)) * 256 + c0) * 128 + head;
+            const float* o0 = scratch.o + (static_cast<int64_t>(div.piece(i, first) * 2 + half) * 256 + c0) * 128 + head;
             const float* o1 =
-                scratch.o + (static_cast<int64_t>(div.piece(i + kStep <= i1 ? i + kStep : i, first)) * 256 + c0) * 128 + head;
+                scratch.o + (static_cast<int64_t>(div.piece(i + kStep <= i1 ? i + kStep : i, first) * 2 + half) * 256 + c0) * 128 + head;
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
                 a[c] = __ldcg(o0 + c * 128);
@@ -684,15 +683,16 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
     }
 }
 
+// Among pairs of CTAs, one for each half of the output columns.
 Division wide_division(int64_t tokens, int64_t topk, int sms) {
-    return Division(2 * tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms);  // no entry: one empty tile
+    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms > 1 ? sms / 2 : 1);  // no entry: an empty tile
 }
 
 // Byte offsets of the scratch arrays; [4] is the size.
 void wide_layout(const Division& d, int64_t tokens, bool weights, int64_t (&at)[5]) {
     at[0] = 0;
-    at[1] = at[0] + align256(2ll * d.ctas * 256 * 4);
-    at[2] = at[1] + align256(2ll * d.ctas * 256 * 128 * 4);
+    at[1] = at[0] + align256(4ll * d.ctas * 256 * 4);
+    at[2] = at[1] + align256(4ll * d.ctas * 256 * 128 * 4);
     at[3] = at[2] + (weights ? align256(tokens * d.tiles * 128 * 4) : 0);
     at[4] = at[3] + (weights ? tokens * d.tiles * 32 * 128 * 4 : 0);
 }
@@ -716,7 +716,7 @@ int launch_wide(cudaStream_t s, const Operands& op, void* workspace) {
     int rc = asu_max_dynamic_smem(reinterpret_cast<const void*>(kv4_decode_wide_kernel), &max_dynamic);
     if (rc != ASU_OK) return rc;
     if (max_dynamic < kWideSmem) return ASU_ERR_ARG;
-    rc = launch_pdl(kv4_decode_wide_kernel, dim3(d.ctas), dim3(kWideThreads), kWideSmem, s, op, d, scratch);
+    rc = launch_pdl(kv4_decode_wide_kernel, dim3(2 * d.ctas), dim3(kWideThreads), kWideSmem, s, op, d, scratch);
     int most = 1;  // pieces of a row
     for (int i = 1; i < d.ctas && most < 3; ++i)
         if (d.start(i) % d.tiles != 0) most = d.start(i + 1) / d.tiles == d.start(i) / d.tiles && i + 1 < d.ctas ? 3 : 2;
