@@ -25,12 +25,14 @@
 // 13 warps: 4 softmax, 8 that load rows into registers and dequantise (the next tile's loads are issued as
 // soon as a tile is stored, and fly during its products), one that issues the products.
 //
-// 128 tokens x 16 heads x 2048 entries take 56 us, 61 x 64 x 1024 35 us.  A tile is a chain of 3.4 us: the
-// output products of its first half 0.35, two halves to dequantise 0.7 to 0.85 each (shared-memory stores: 128
-// KB are 1000 cycles), the scores' second half 0.45, the softmax 0.45, four hand-overs of 0.15; the loads of
-// rows are hidden.  Tried and slower: tiles of 64 entries twice (both buffers are held while one is filled:
-// 78 us), rows through asynchronous copies and 16 warps that dequantise and make the softmax (62 us), products
-// of single warps with rows dequantised in registers (79 us).
+// 128 tokens x 16 heads x 2048 entries take 55 us, 61 x 64 x 1024 32 us, of which the joining of the pieces 6 and 8.
+// A tile is a chain of 3.3 us: the output products of its first half 0.35, two halves to dequantise 0.7 to 0.85
+// each (shared memory: 128 KB stored, and the products' rows read at the same time), the scores' second half 0.45,
+// the softmax 0.45, four hand-overs of 0.15; the loads of rows are hidden.  Tried and slower, 16 heads: tiles of 64
+// entries twice (both buffers are held while one is filled: 78 us); rows through asynchronous copies and 16 warps
+// that dequantise and make the softmax (62 us); four quarters instead of two halves (58 us: loads of 32 bytes a
+// row instead of 128); every tile dequantised twice, into tensor memory for the scores (99 us: instructions and
+// loads); products of single warps with rows dequantised in registers (79 us).
 #include "kv4_decode.cuh"
 #include "tcgen05.cuh"
 

@@ -29,12 +29,13 @@ namespace {
 // The running maximum only moves when it grows by more than 2^8: until then the weights stay below
 // 2^8, as exact in bf16 as any others, and the output needs no rescaling.
 //
-// The two halves of a token follow one another, so that every other row of work finds its q in place.
+// The two CTAs of a pair walk the same tiles, so that the rows' second reading finds them in L2.
 //
-// 128 tokens x 128 heads x 2048 entries take 122 us, with weights 143.  A tile takes 1.7 us, of which the
-// products are 1.0 and the traffic of shared memory 1.3; a change of tokens 6 us (the next q's 147 KB, the
-// output through the lanes), the start 6 us; the joining of the pieces 9, with the weights' way through memory
-// and back 23.
+// 128 tokens x 128 heads x 2048 entries take 120 us, with weights 144.  A tile takes 1.7 us, in which the
+// issuing lane waits for the products and for nothing else: they would take 1.0 alone, but the traffic of shared
+// memory is 1.3 (q read again for every tile 0.4, rows dequantised 0.3 and read 0.4, 4-bit rows in and out 0.2).
+// A change of tokens takes 4 us (the next q's 147 KB, the output through the lanes), the start 5, the joining of
+// the pieces 9, with the weights' way through memory and back 23.
 constexpr int kTile = 64;  // entries a tile
 constexpr int kWideThreads = 15 * 32;
 constexpr int kBlock = kTile * 128;  // bytes of a [64 x 64] bf16 block
