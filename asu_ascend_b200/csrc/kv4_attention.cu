@@ -33,16 +33,18 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
                                  int64_t workspace_size, int32_t* status) {
     if (tokens < 0 || heads < 0 || topk < 0 || tokens > ASU_KV4_MAX_TOKENS || heads > ASU_KV4_MAX_HEADS ||
         topk > ASU_KV4_MAX_TOPK || pool_rows < 0 || pool_rows > 0x7fffffff || q_token_stride < 0 || q_head_stride < 0 ||
-        slots_token_stride < 0 || pool_pitch < static_cast<uint64_t>(kRowBytes) || !(scale > 0.0f) ||
-        !(scale < INFINITY))
+        slots_token_stride < 0 || pool_pitch < static_cast<uint64_t>(kRowBytes))
         return ASU_ERR_ARG;
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale_log2 > 0.0f) || !(scale_log2 < INFINITY)) return ASU_ERR_ARG;
     if (tokens == 0 || heads == 0) return ASU_OK;
     if (!q || !out || !lse || (topk && (!slots || !pool))) return ASU_ERR_ARG;
     const int64_t need = decode_workspace(tokens, heads, topk, weights != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_size < need)) return ASU_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(pool) % 16 || pool_pitch % 16 ||
         pool_token_stride % 16 || reinterpret_cast<uintptr_t>(out) % 32 || reinterpret_cast<uintptr_t>(lse) % 4 ||
-        reinterpret_cast<uintptr_t>(workspace) % 32)
+        reinterpret_cast<uintptr_t>(workspace) % 32 || reinterpret_cast<uintptr_t>(slots) % 4 ||
+        reinterpret_cast<uintptr_t>(weights) % 2)
         return ASU_ERR_ALIGN;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Operands op;
@@ -58,7 +60,7 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     op.tokens = static_cast<int32_t>(tokens);
     op.heads = static_cast<int32_t>(heads);
     op.topk = static_cast<int32_t>(topk);
-    op.scale_log2 = scale * 1.4426950408889634f;
+    op.scale_log2 = scale_log2;
     op.q_aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     op.out = static_cast<__nv_bfloat16*>(out);
     op.lse = lse;

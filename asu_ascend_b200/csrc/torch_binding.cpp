@@ -555,7 +555,8 @@ void kv4_decode_checks(const at::Tensor& q, const at::Tensor& pool, const at::Te
     TORCH_CHECK(slots.dim() == 2 && slots.size(0) == q.size(0), "slots must be [tokens, topk], got ", slots.sizes());
     TORCH_CHECK(slots.stride(1) == 1 || slots.size(1) <= 1 || slots.size(0) == 0, "slots rows must be contiguous");
     TORCH_CHECK(slots.size(1) <= ASU_KV4_MAX_TOPK, "at most 16384 entries a token, got ", slots.size(1));
-    TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0.0f,
+    // (the kernels multiply it by log2(e))
+    TORCH_CHECK_VALUE(scale > 0.0 && static_cast<float>(scale) > 0.0f && std::isfinite(static_cast<float>(scale) * 1.4426950408889634f),
                       "scale must be positive and finite");
 }
 

@@ -124,7 +124,7 @@ class WeightSlotPools:
         if keep_from is not None and (keep_from.dtype != torch.int32 or keep_from.device != dev
                                       or tuple(keep_from.shape) != (R,) or not keep_from.is_contiguous()):
             raise RuntimeError(f"keep_from must be a contiguous int32 tensor [{R}] on the pool's device")
-        o = out or self._out
+        o = self._out if out is None else self._checked(out)
         s = (stream or torch.cuda.current_stream(dev)).cuda_stream
         with torch.cuda.device(dev):
             check(lib.asu_weight_step(
@@ -135,6 +135,17 @@ class WeightSlotPools:
                 o.evicted_count.data_ptr(), self.stats.data_ptr(), self.status.data_ptr(), R, self.key_space,
                 self.slot_count, self.query_count, self.free_target), "asu_weight_step")
         return o
+
+    def _checked(self, out: LruStepOutput) -> LruStepOutput:
+        R, Q = self.req_num, self.query_count
+        for name, shape, dtype in (("slot", (R, Q), torch.int32), ("hit", (R, Q), torch.bool), ("install", (R, Q), torch.bool),
+                                   ("evicted", None, torch.int32), ("evicted_count", (R,), torch.int32)):
+            t = getattr(out, name)
+            if name == "evicted":
+                shape = (R, max(t.shape[-1], self.free_target, 1))
+            if tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
+                raise RuntimeError(f"out.{name} must be one of new_output()'s: contiguous {dtype} on the pool's device")
+        return out
 
     def check_status(self, ignore: int = ST_SHORTAGE) -> None:
         raise_on_status(self.status, "asu_weight_step", ignore)

@@ -142,8 +142,9 @@ def test_rows_that_cannot_be_stored_are_reported(kv4):
 
 # ---- attention ---------------------------------------------------------------------------------
 
-def check(q, pool, slots, scale, got):
-    """got against the oracle, token by token; q a CPU bf16 tensor, pool / slots numpy arrays."""
+def check(q, pool, slots, scale, got, lost=0.0):
+    """got against the oracle, token by token; q a CPU bf16 tensor, pool / slots numpy arrays; `lost`: what the
+    outputs may be off by for weights below the range of the exponent, relative to the largest value."""
     out = got.out.float().cpu().numpy().astype(np.float64)
     lse = got.lse.cpu().numpy().astype(np.float64)
     w = None if got.weights is None else got.weights.float().cpu().numpy().astype(np.float64)
@@ -153,6 +154,8 @@ def check(q, pool, slots, scale, got):
         ds = (576 * 2.0**-23 + 2.0**-22) * smag
         lim = (H_BF16 + 2 * ds[:, None] + 2 * 2.0**-16) * mag
         lim += H_BF16 * (np.abs(o) + lim)
+        if lost:
+            lim += lost * np.abs(O.unpack(p)[:, :512]).max()
         worst = np.abs(out[t] - o) - lim
         assert (worst <= 0).all(), (t, np.argwhere(worst > 0)[:4], worst.max())
         if np.isinf(l).any():
@@ -267,6 +270,27 @@ def test_large_scores_do_not_overflow(kv4, checked, H):
     got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 1.0, weights=True)
     assert torch.isfinite(got.out.float()).all() and torch.isfinite(got.lse).all()
     check(q, pool, slots, 1.0, got)
+
+
+@pytest.mark.parametrize("H,loud", [(16, 60.0), (24, 60.0), (64, 60.0), (128, 60.0), (16, 3.0), (64, 3.0), (128, 3.0)])
+def test_scores_that_rise_from_tile_to_tile(kv4, checked, H, loud):
+    """Enough tokens that one block walks several tiles of each, in the order of one head's scores, upwards or
+    downwards: what was summed so far has to be scaled again and again, after tiles without any entry too."""
+    T, K, S = 170, 500, 520
+    q, pool, slots = case(T, H, K, S, False, 19, 0.97, loud)
+    kv = O.unpack(pool)
+    for t in range(T):
+        s = kv[slots[t]] @ q[t, t % H].double().numpy()
+        s[slots[t] < 0] = s.min()
+        slots[t] = slots[t][np.argsort(s if t % 3 else -s)]
+        if t % 5 == 0:
+            slots[t, : 64 * (t % 4 + 1)] = -1
+    got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 1.0, weights=True)
+    # Scores this far apart leave outputs of 1e-30 where the large weights' values are 0 or cancel.  The
+    # exponentials are relative to a score of the token, so their sum is at least 1; one below 2^-126 may count as 0,
+    # and its bf16 form be off by half of the smallest step, 2^-134: K entries lose at most K (2^-126 + 2^-134) max|v|.
+    # The output's own smallest step adds 2^-134, less than 2^-126 of the largest value.
+    check(q, pool, slots, 1.0, got, K * 2.0**-125)
 
 
 @pytest.mark.parametrize("H,qpad,qoff", [(16, 64, 0), (16, 0, 3), (128, 64, 0), (128, 8, 5), (40, 0, 1)])

@@ -146,6 +146,57 @@ def test_step_refuses_wrong_tensors(WeightSlotPools):
             pools.step(*args, **kw)
 
 
+def test_step_refuses_output_buffers_of_other_pools(WeightSlotPools):
+    pools = WeightSlotPools(2, 100, 16, 4, 8, device=DEV)
+    q = torch.zeros(2, 8, dtype=torch.int32, device=DEV)
+    pools.step(q, out=pools.new_output())
+    for other in (WeightSlotPools(2, 100, 16, 4, 7, device=DEV), WeightSlotPools(1, 100, 16, 4, 8, device=DEV),
+                  WeightSlotPools(2, 100, 16, 3, 8, device=DEV)):
+        with pytest.raises(RuntimeError, match="new_output"):
+            pools.step(q, out=other.new_output())
+    out = pools.new_output()
+    out.hit = out.hit.to(torch.int32)
+    with pytest.raises(RuntimeError, match="out.hit"):
+        pools.step(q, out=out)
+
+
+@pytest.mark.parametrize("n,names", [(4096, 1), (4096, 3), (1500, 700), (33, 2)])
+def test_many_weights_of_one_slot_add_up_in_their_order(WeightSlotPools, n, names):
+    """Every rounding counts: weights of many sizes, and the sum in the entries' order bit for bit."""
+    S = 1024
+    pools = WeightSlotPools(1, 5000, S, 0, 1024, decay=0.75, device=DEV)
+    keys = torch.arange(S, dtype=torch.int32, device=DEV).view(1, S)
+    pools.step(keys)
+    rng = np.random.default_rng(n + names)
+    pools.score.copy_(torch.from_numpy(rng.random((1, S)).astype(np.float32)))
+    score = (pools.score[0].cpu().numpy() * np.float32(0.75)).astype(np.float32)
+    last = rng.permutation(S)[:names][rng.integers(0, names, n)].astype(np.int32)
+    w = np.exp2(rng.uniform(-20, 3, n)).astype(np.float32)
+    for s, x in zip(last, w):
+        score[s] = np.float32(score[s] + x)
+    pools.step(keys, torch.from_numpy(last).view(1, n).to(DEV), torch.from_numpy(w).view(1, n).to(DEV))
+    assert np.array_equal(pools.score[0].cpu().numpy().view(np.uint32), score.view(np.uint32))
+    pools.check_status()
+
+
+def test_scores_that_cannot_be_count_as_zero_and_are_reported(WeightSlotPools):
+    """Negative and NaN scores of a state that someone else wrote: the lowest, by slot, and the status says so;
+    infinite ones are the last to leave."""
+    pools = WeightSlotPools(1, 100, 8, 3, 8, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    pools.step(torch.arange(8, **i32).view(1, 8))
+    pools.score.copy_(torch.tensor([[float("inf"), 1.0, -3.0, 2.0, float("nan"), -0.0, 0.5, float("inf")]], device=DEV))
+    out = pools.step(torch.full((1, 8), 50, **i32))
+    assert out.evicted[0].tolist() == [2, 4, 5] and int(out.evicted_count) == 3
+    assert pools.score[0].tolist() == [float("inf"), 1, 0, 2, 0, 0, 0.5, float("inf")]
+    with pytest.raises(RuntimeError, match="BAD_STATE"):
+        pools.check_status()
+    pools.status.zero_()
+    pools.score.copy_(torch.full((1, 8), float("inf"), device=DEV))
+    out = pools.step(torch.full((1, 8), 60, **i32))
+    assert int(out.evicted_count) == 1 and out.evicted[0, 0] == 0  # free 2 of 3: one more, the lowest slot
+
+
 def test_graph_replay_and_the_step_writing_over_its_last_slots(WeightSlotPools):
     """One captured step whose last_slot is its own output buffer, against eager steps with copies."""
     R, K, S, Q, target = 3, 2000, 256, 64, 80

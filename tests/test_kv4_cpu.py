@@ -103,6 +103,14 @@ def test_attention_rejects_before_launch(lib):
     assert size(0, 16, 2048, 0) >= 0
 
 
+def test_attention_rejects_what_its_vector_stores_and_scaling_cannot_take(lib):
+    L, A, G = lib.lib, lib.ASU_ERR_ARG, lib.ASU_ERR_ALIGN
+    ok = dict(out=64, ws=64)
+    for bad in (dict(out=48), dict(ws=48), dict(slots=18), dict(weights=17)):
+        assert _attention(L, **(ok | bad)) == G, bad
+    assert _attention(L, **ok, scale=3e38) == A  # times log2(e) it is infinite
+
+
 def _step(L, **kw):
     a = dict(stream=None, t2s=16, s2t=16, score=16, stack=16, count=16, last=1 << 20, weight=16, wtype=2, n=4, decay=0.5,
              keep=None, query=16, slot=1 << 30, hit=16, inst=16, ev=16, ev_stride=4, evn=16, stats=None, status=None,
@@ -161,7 +169,7 @@ def test_torch_operators_check_their_arguments_on_host_tensors():
                        ((q, pool, torch.zeros(5, 2, dtype=i32).t(), 1.0), "rows must be contiguous"),
                        ((q, pool, torch.zeros(2, 16385, dtype=i32), 1.0), "16384"),
                        ((q, pool, sl, float("inf")), "scale"), ((q, pool, sl, 0.0), "scale"),
-                       ((q, pool, sl, 1e-60), "scale"),
+                       ((q, pool, sl, 1e-60), "scale"), ((q, pool, sl, 3e38), "scale"),
                        ((q.clone().requires_grad_(), pool, sl, 1.0), "requires a gradient"),
                        ((q, pool, sl, 1.0), "needs CUDA")):
         with pytest.raises((RuntimeError, ValueError), match=text):
