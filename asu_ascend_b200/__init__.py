@@ -13,6 +13,8 @@ if it is not built -- there is no CPU fallback):
 * ``kv_server``         MicroKV socket protocol in front of that store
 * ``hbm_lookup_update`` mirror of the reference's gather/update extension module
 * ``lru``               per-request exact-LRU slot pools (LruSlotPools)
+* ``weight_pools``      slot pools that evict by accumulated attention weight (WeightSlotPools)
+* ``kv4``               416-byte rows of 4-bit latents, and sparse attention over them
 * ``host_pool``         pinned mapped host row pool + swap-in gather (HostRowPool)
 * ``dist``              request sharding, end-of-run statistics, rank placement on a host's GPUs
 * ``balance``           swap-in balancing between the ranks of one host (peer stores over NVLink)
