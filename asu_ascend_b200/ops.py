@@ -27,6 +27,8 @@ from pathlib import Path
 
 import torch
 
+from ._lib import _SIGS
+
 NAMESPACES = ("asu", "_C_ascend")
 
 _STATUS_CHECKS = os.environ.get("ASU_CHECK_STATUS", "0") not in ("", "0")
@@ -44,10 +46,17 @@ def _load_torch_binding() -> ctypes.CDLL:
     handle = ctypes.CDLL(str(TORCH_LIB_PATH))  # the same loaded image: shares the status-check flag
     handle.asu_torch_set_status_checks.argtypes = [ctypes.c_int]
     handle.asu_torch_set_status_checks.restype = None
+    handle.asu_torch_weight_step.argtypes = [ctypes.c_int, ctypes.c_int, *_SIGS["asu_weight_step"]]
+    handle.asu_torch_weight_step.restype = ctypes.c_int
     return handle
 
 
 _torch_binding = _load_torch_binding()
+
+
+def weight_step(*args) -> int:
+    """``asu_weight_step`` with (device, whether a stream is given, stream) in the place of the stream."""
+    return _torch_binding.asu_torch_weight_step(*args)
 
 
 def set_status_checks(enabled: bool) -> None:

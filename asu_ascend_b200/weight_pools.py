@@ -12,8 +12,9 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import DTYPE_BF16, DTYPE_FP32, LRU_STAT_COLS, ST_SHORTAGE, check, lib, raise_on_status
+from ._lib import DTYPE_BF16, DTYPE_FP32, LRU_STAT_COLS, ST_SHORTAGE, check, raise_on_status
 from .lru import LruStepOutput
+from .ops import weight_step
 
 _WEIGHT_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_FP32}
 
@@ -105,35 +106,34 @@ class WeightSlotPools:
         dev, R = self.device, self.req_num
         if query.dtype != torch.int32 or query.device != dev or not query.is_contiguous():
             raise RuntimeError("query must be a contiguous int32 tensor on the pool's device")
-        if tuple(query.shape) != (R, self.query_count):
+        if query.shape != (R, self.query_count):
             raise RuntimeError(f"query must be [{R}, {self.query_count}], got {tuple(query.shape)}")
         n, wtype, lptr, wptr = 0, DTYPE_FP32, None, None
-        if (last_slot is None) != (last_weight is None):
-            raise RuntimeError("last_slot and last_weight go together")
-        if last_slot is not None:
+        if last_slot is not None and last_weight is not None:
             if last_slot.dtype != torch.int32 or last_slot.device != dev or not last_slot.is_contiguous():
                 raise RuntimeError("last_slot must be a contiguous int32 tensor on the pool's device")
             wtype = _WEIGHT_DTYPES.get(last_weight.dtype)
             if wtype is None or last_weight.device != dev or not last_weight.is_contiguous():
                 raise RuntimeError("last_weight must be a contiguous bfloat16 or float32 tensor on the pool's device")
-            if last_slot.dim() != 2 or last_slot.shape[0] != R or last_weight.shape != last_slot.shape:
+            shape = last_slot.shape
+            if len(shape) != 2 or shape[0] != R or last_weight.shape != shape:
                 raise RuntimeError(f"last_slot and last_weight must both be [{R}, n]")
-            n, lptr, wptr = last_slot.shape[1], last_slot.data_ptr(), last_weight.data_ptr()
+            n, lptr, wptr = shape[1], last_slot.data_ptr(), last_weight.data_ptr()
             if n > 4096:
                 raise RuntimeError(f"at most 4096 weights a request, got {n}")
+        elif last_slot is not None or last_weight is not None:
+            raise RuntimeError("last_slot and last_weight go together")
         if keep_from is not None and (keep_from.dtype != torch.int32 or keep_from.device != dev
-                                      or tuple(keep_from.shape) != (R,) or not keep_from.is_contiguous()):
+                                      or keep_from.shape != (R,) or not keep_from.is_contiguous()):
             raise RuntimeError(f"keep_from must be a contiguous int32 tensor [{R}] on the pool's device")
         o = self._out if out is None else self._checked(out)
-        s = (stream or torch.cuda.current_stream(dev)).cuda_stream
-        with torch.cuda.device(dev):
-            check(lib.asu_weight_step(
-                s, self.token_to_slot.data_ptr(), self.slot_to_token.data_ptr(), self.score.data_ptr(),
-                self.free_stack.data_ptr(), self.free_count.data_ptr(), lptr, wptr, wtype, n, self.decay,
-                None if keep_from is None else keep_from.data_ptr(), query.data_ptr(), o.slot.data_ptr(),
-                o.hit.data_ptr(), o.install.data_ptr(), o.evicted.data_ptr(), o.evicted.shape[1],
-                o.evicted_count.data_ptr(), self.stats.data_ptr(), self.status.data_ptr(), R, self.key_space,
-                self.slot_count, self.query_count, self.free_target), "asu_weight_step")
+        check(weight_step(
+            dev.index, stream is not None, None if stream is None else stream.cuda_stream, self.token_to_slot.data_ptr(),
+            self.slot_to_token.data_ptr(), self.score.data_ptr(), self.free_stack.data_ptr(), self.free_count.data_ptr(),
+            lptr, wptr, wtype, n, self.decay, None if keep_from is None else keep_from.data_ptr(), query.data_ptr(),
+            o.slot.data_ptr(), o.hit.data_ptr(), o.install.data_ptr(), o.evicted.data_ptr(), o.evicted.shape[1],
+            o.evicted_count.data_ptr(), self.stats.data_ptr(), self.status.data_ptr(), R, self.key_space,
+            self.slot_count, self.query_count, self.free_target), "asu_weight_step")
         return o
 
     def _checked(self, out: LruStepOutput) -> LruStepOutput:
