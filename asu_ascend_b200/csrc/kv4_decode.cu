@@ -589,7 +589,7 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
 int columns_of(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
 Division division(int64_t tokens, int64_t topk, int sms) {
-    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms);  // no entry: one empty tile
+    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms, 1);  // no entry: one empty tile
 }
 
 void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {

@@ -24,29 +24,48 @@ struct Operands {
     int32_t* status;
 };
 
-// Row (token of one part of the call) r has `tiles` consecutive units; CTA i takes the units
-// [start(i), start(i + 1)), `each` of them and one more in the first `more` CTAs.  A row that lies in
-// several CTAs' ranges is joined afterwards.  The division depends on the call's sizes alone, so results
+// Row (token) r has `tiles` consecutive units; CTA i takes the units [start(i), start(i + 1)).  Either all CTAs take
+// the same number of units, `each` and one more in the first `more` of them, wherever rows begin and end; or every row
+// is cut in `parts` of `each` units (the last may be shorter) and a CTA takes one.  Both end when the CTA with the most
+// units does; the second spares CTAs a change of rows in the middle of their range (q, the output), which costs as
+// much as `change` units, and leaves fewer pieces to join.  It depends on the call's sizes alone, so results
 // repeat.  All in 32 bits: 64-bit divisions were a third of the kernels' code.
 struct Division {
-    int32_t rows, tiles, ctas, each, more;
+    int32_t rows, tiles, ctas, each, more, parts;  // parts 0: the first kind
     Division() = default;
-    Division(int64_t rows_, int64_t tiles_, int64_t most) {
+    Division(int64_t rows_, int64_t tiles_, int64_t most, int64_t change) {
         rows = static_cast<int32_t>(rows_);
         tiles = static_cast<int32_t>(tiles_);
         const int64_t units = rows_ * tiles_;  // below 2^26: tokens, entries and parts are bounded
         ctas = static_cast<int32_t>(units < most ? units : most);
         each = static_cast<int32_t>(units / ctas);
         more = static_cast<int32_t>(units % ctas);
+        parts = 0;
+        if (rows_ <= most) {
+            int64_t cut = most / rows_ < tiles_ ? most / rows_ : tiles_;
+            const int64_t per = (tiles_ + cut - 1) / cut;
+            if (per <= each + (more > 0) + change) {
+                cut = (tiles_ + per - 1) / per;
+                parts = static_cast<int32_t>(cut);
+                each = static_cast<int32_t>(per);
+                ctas = static_cast<int32_t>(rows_ * cut);
+                more = 0;
+            }
+        }
     }
-    __host__ __device__ __forceinline__ int32_t start(int32_t i) const { return i * each + (i < more ? i : more); }
+    __host__ __device__ __forceinline__ int32_t start(int32_t i) const {
+        if (parts > 0) return i / parts * tiles + i % parts * each;
+        return i * each + (i < more ? i : more);
+    }
     __host__ __device__ __forceinline__ int32_t cta_of(int32_t u) const {
+        if (parts > 0) return u / tiles * parts + u % tiles / each;
         const int32_t first = more * (each + 1);
         return u < first ? u / (each + 1) : more + (u - first) / each;
     }
     // Scratch slot of CTA i's piece of a row that starts at unit `row_start`: a CTA's range holds at
     // most two pieces of rows, one at its start and one at its end.
     __host__ __device__ __forceinline__ int32_t piece(int32_t i, int32_t row_start) const {
+        if (parts > 0) return 2 * i;
         return 2 * i + (start(i) >= row_start ? 0 : 1);
     }
 };

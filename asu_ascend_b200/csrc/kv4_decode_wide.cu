@@ -686,7 +686,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
 
 // Among pairs of CTAs, one for each half of the output columns.
 Division wide_division(int64_t tokens, int64_t topk, int sms) {
-    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms > 1 ? sms / 2 : 1);  // no entry: an empty tile
+    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms > 1 ? sms / 2 : 1, 3);  // no entry: an empty tile
 }
 
 // Byte offsets of the scratch arrays; [4] is the size.
