@@ -25,7 +25,11 @@
 // 13 warps: 4 softmax, 8 that load rows into registers and dequantise (the next tile's loads are issued as
 // soon as a tile is stored, and fly during its products), one that issues the products.
 //
-// 128 tokens x 16 heads x 2048 entries take 55 us, 61 x 64 x 1024 32 us, of which the joining of the pieces 6 and 8.
+// Tokens cut into 2 to 8 equal parts are joined by the cluster of their CTAs, if all clusters run at once: 61 x 64 x
+// 1024 31.1 -> 29.4 us, 32 x 32 x 2048 22.1 -> 20.8, with weights of an uncut token 1 x 16 x 100 13.5 -> 12.3.  Others
+// are joined by a second kernel, 5 to 8 us after the first.
+//
+// 128 tokens x 16 heads x 2048 entries take 55 us, 61 x 64 x 1024 29 us.
 // A tile is a chain of 3.3 us: the output products of its first half 0.35, two halves to dequantise 0.7 to 0.85
 // each (shared memory: 128 KB stored, and the products' rows read at the same time), the scores' second half 0.45,
 // the softmax 0.45, four hand-overs of 0.15; the loads of rows are hidden.  Tried and slower, 16 heads: tiles of 64
@@ -33,6 +37,8 @@
 // that dequantise and make the softmax (62 us); four quarters instead of two halves (58 us: loads of 32 bytes a
 // row instead of 128); every tile dequantised twice, into tensor memory for the scores (99 us: instructions and
 // loads); products of single warps with rows dequantised in registers (79 us).
+#include <atomic>
+
 #include "kv4_decode.cuh"
 #include "tcgen05.cuh"
 
@@ -44,6 +50,7 @@ constexpr int kThreads = 13 * 32;
 constexpr int kTile = 128;
 constexpr int kBlock = kTile * 128;  // bytes of a [128 entries x 64] block
 constexpr float kMaxGrowth = 40.0f;  // base 2
+constexpr int kMaxParts = 8;         // CTAs of a cluster
 
 // Every barrier is waited for in every phase by each of its waiters, and its next phase depends on them: a
 // phase is never two ahead of one that waits for it.
@@ -108,7 +115,100 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 
+// A token's CTAs are a cluster: when all have written their pieces, each joins a share of the heads and sums the
+// weights of its own tiles.  That spares the second launch and its way to every SM.  `smem` is free: [9][kN] factors
+// of the pieces and lse, and [3][kN] of a tile's weights.
 template <int kN>
+__device__ __forceinline__ void join_in_cluster(const Operands& op, const Division& div, const Scratch& scratch,
+                                                float* smem) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int parts = div.parts, token = blockIdx.x / parts, rank = blockIdx.x % parts;
+    const int first_cta = token * parts;
+    float(*s_factor)[kN] = reinterpret_cast<float(*)[kN]>(smem);
+    float* s_lse = s_factor[kMaxParts];  // base 2
+    if (parts == 1) {  // the outputs are written, and only weights are asked for
+        if (threadIdx.x < kN)
+            s_lse[threadIdx.x] = static_cast<int>(threadIdx.x) < op.heads
+                                     ? op.lse[static_cast<int64_t>(token) * op.heads + threadIdx.x] * 1.4426950408889634f
+                                     : -INFINITY;
+    } else if (threadIdx.x < kN) {
+        const int h = threadIdx.x;
+        float m[kMaxParts], l[kMaxParts], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kMaxParts; ++p) {
+            const float* ml = scratch.ml + 4 * (first_cta + (p < parts ? p : 0)) * kN + h;
+            m[p] = p < parts ? __ldcg(ml) : -INFINITY;
+            l[p] = __ldcg(ml + kN);
+            top = fmaxf(top, m[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < kMaxParts; ++p) {
+            m[p] = m[p] == -INFINITY ? 0.0f : exp2_fast(m[p] - top);
+            sum = fmaf(l[p], m[p], sum);
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int p = 0; p < kMaxParts; ++p) s_factor[p][h] = m[p] * inv;
+        s_lse[h] = sum > 0.0f && h < op.heads ? top + log2f(sum) : -INFINITY;
+        if (rank == 0 && h < op.heads)
+            op.lse[static_cast<int64_t>(token) * op.heads + h] =
+                sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+    __syncthreads();
+    const int t = threadIdx.x & 127, group = threadIdx.x >> 7;  // three groups, and a warp that looks on
+    if (group >= 3) return;
+    constexpr int kHeads = 4;  // at a time: their loads fly together
+    const int share = (op.heads + parts - 1) / parts;
+    const int last = min(op.heads, (rank + 1) * share);
+    for (int h0 = rank * share + group * kHeads; parts > 1 && h0 < last; h0 += 3 * kHeads) {
+        float4 acc[kHeads] = {};
+#pragma unroll 2
+        for (int p = 0; p < parts; ++p) {
+            float4 v[kHeads];
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k)
+                v[k] = __ldcg(reinterpret_cast<const float4*>(
+                                  scratch.o + (static_cast<int64_t>(2 * (first_cta + p)) * kN + min(h0 + k, last - 1)) * kLatent) + t);
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) {
+                const float f = s_factor[p][min(h0 + k, last - 1)];
+                acc[k].x = fmaf(v[k].x, f, acc[k].x), acc[k].y = fmaf(v[k].y, f, acc[k].y);
+                acc[k].z = fmaf(v[k].z, f, acc[k].z), acc[k].w = fmaf(v[k].w, f, acc[k].w);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k)
+            if (h0 + k < last)
+                reinterpret_cast<uint2*>(op.out + (static_cast<int64_t>(token) * op.heads + h0 + k) * kLatent)[t] =
+                    make_uint2(pack_bf16(acc[k].x, acc[k].y), pack_bf16(acc[k].z, acc[k].w));
+    }
+    if (op.weights == nullptr) return;
+    float* s_tile = s_factor[kMaxParts + 1 + group];
+    for (int u = div.start(blockIdx.x) + group; u < div.start(blockIdx.x + 1); u += 3) {
+        const uint4* p = reinterpret_cast<const uint4*>(scratch.p + (static_cast<int64_t>(u) * kTile + t) * kN);
+        uint4 v[kN / 8];
+#pragma unroll
+        for (int i = 0; i < kN / 8; ++i) v[i] = __ldcg(p + i);
+        if (t < kN) s_tile[t] = s_lse[t] == -INFINITY ? 0.0f : exp2_fast(__ldcg(scratch.ref + static_cast<int64_t>(u) * kN + t) - s_lse[t]);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+        const int e = (u - token * div.tiles) * kTile + t;
+        float w = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kN / 8; ++i) {
+            const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w = fmaf(__uint_as_float(x[k] << 16), s_tile[i * 8 + 2 * k], w);
+                w = fmaf(__uint_as_float(x[k] & 0xffff0000u), s_tile[i * 8 + 2 * k + 1], w);
+            }
+        }
+        if (e < op.topk) op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(w);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+    }
+}
+
+// kJoin: a token's CTAs are a cluster and join their pieces themselves.
+template <int kN, bool kJoin>
 __global__ void __launch_bounds__(kThreads, 1)
 kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) {
     using L = Layout<kN>;
@@ -463,6 +563,10 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         }
     }
     pdl_trigger();
+    if constexpr (kJoin) {
+        __syncwarp();
+        join_in_cluster<kN>(op, div, scratch, reinterpret_cast<float*>(smem_raw));
+    }
     __syncthreads();
     if (s_dead && tid == 0) flag_status(op.status, 0, ASU_ST_TIMEOUT);
     if (warp == 12) {
@@ -601,6 +705,32 @@ void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
     at[4] = at[3] + (weights ? units * kTile * n * 2 : 0);
 }
 
+// How many clusters of that many CTAs the device can run at once; asked once per device.
+template <int kN>
+int most_clusters(int parts) {
+    static std::atomic<int> known[64][kMaxParts + 1];  // 1 + the answer
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int n = known[dev][parts].load(std::memory_order_relaxed) - 1;
+    if (n >= 0) return n;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(parts);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(parts));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Layout<kN>::kBytes;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kv4_decode_kernel<kN, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    known[dev][parts].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
 template <int kN>
 int launch(cudaStream_t s, const Operands& op, void* workspace) {
     const Division d = division(op.tokens, op.topk, asu_sm_count());
@@ -610,10 +740,17 @@ int launch(cudaStream_t s, const Operands& op, void* workspace) {
     const Scratch scratch = {reinterpret_cast<float*>(ws + at[0]), reinterpret_cast<float*>(ws + at[1]),
                              reinterpret_cast<float*>(ws + at[2]), reinterpret_cast<__nv_bfloat16*>(ws + at[3])};
     int max_dynamic = 0;
-    int rc = asu_max_dynamic_smem(reinterpret_cast<const void*>(kv4_decode_kernel<kN>), &max_dynamic);
+    int rc = asu_max_dynamic_smem(reinterpret_cast<const void*>(kv4_decode_kernel<kN, false>), &max_dynamic);
     if (rc != ASU_OK) return rc;
     if (max_dynamic < Layout<kN>::kBytes) return ASU_ERR_ARG;
-    rc = launch_pdl(kv4_decode_kernel<kN>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s, op, d, scratch);
+    if (d.parts > (op.weights != nullptr ? 0 : 1) && d.parts <= kMaxParts) {
+        rc = asu_max_dynamic_smem(reinterpret_cast<const void*>(kv4_decode_kernel<kN, true>), &max_dynamic);
+        if (rc != ASU_OK) return rc;
+        if (max_dynamic >= Layout<kN>::kBytes && most_clusters<kN>(d.parts) >= op.tokens)
+            return launch_pdl_clusters(kv4_decode_kernel<kN, true>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s,
+                                       static_cast<unsigned>(d.parts), op, d, scratch);
+    }
+    rc = launch_pdl(kv4_decode_kernel<kN, false>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s, op, d, scratch);
     bool shared_rows = false;  // does any row lie in several CTAs' ranges?
     for (int i = 1; i < d.ctas && !shared_rows; ++i) shared_rows = d.start(i) % d.tiles != 0;
     if (rc != ASU_OK || (!shared_rows && op.weights == nullptr)) return rc;
