@@ -10,11 +10,11 @@ using namespace asu;
 using namespace asu::kv4;
 
 // Up to kTallHeads heads the kernel whose products have the heads as columns, above it the one whose products
-// have them as 128 rows.  One and the other in us, 2048 entries:
-//   heads            16        32        64        80       128
-//   128 tokens  52 / 115  64 / 116  95 / 118  167 / 120  181 / 125
-//   32 tokens   22 /  57  26 /  57  35 /  58   54 /  58   56 /  59
-//   1 token     17 /  17  17 /  17  18 /  16   19 /  16   18 /  16
+// have them as 128 rows.  One and the other in us, 2048 entries (in brackets the heads taken 64 at a time):
+//   heads             16        32        64          80         128
+//   128 tokens  51 / 109  59 / 110  90 / 112  (167) / 113  (181) / 117
+//   32 tokens   20 /  37  21 /  37  30 /  38   (54) /  38   (56) /  39
+// For one token they are within 2 us of each other.
 static int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
     return heads <= kTallHeads ? tall_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
 }
