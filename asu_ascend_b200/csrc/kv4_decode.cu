@@ -707,7 +707,7 @@ void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
 
 // How many clusters of that many CTAs the device can run at once; asked once per device.
 template <int kN>
-int most_clusters(int parts) {
+int most_clusters(int parts, int bytes) {
     static std::atomic<int> known[64][kMaxParts + 1];  // 1 + the answer
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
@@ -720,7 +720,7 @@ int most_clusters(int parts) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(parts));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Layout<kN>::kBytes;
+    cfg.dynamicSmemBytes = bytes;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, kv4_decode_kernel<kN, true>, &cfg) != cudaSuccess) {
@@ -746,8 +746,10 @@ int launch(cudaStream_t s, const Operands& op, void* workspace) {
     if (d.parts > (op.weights != nullptr ? 0 : 1) && d.parts <= kMaxParts) {
         rc = asu_max_dynamic_smem(reinterpret_cast<const void*>(kv4_decode_kernel<kN, true>), &max_dynamic);
         if (rc != ASU_OK) return rc;
-        if (max_dynamic >= Layout<kN>::kBytes && most_clusters<kN>(d.parts) >= op.tokens)
-            return launch_pdl_clusters(kv4_decode_kernel<kN, true>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s,
+        // All of the SM's shared memory: blocks of a cluster wait for one another while they hold tensor memory, which
+        // another kernel's cluster on the same SMs must not wait for while it holds some.
+        if (max_dynamic >= Layout<kN>::kBytes && most_clusters<kN>(d.parts, max_dynamic) >= op.tokens)
+            return launch_pdl_clusters(kv4_decode_kernel<kN, true>, dim3(d.ctas), dim3(kThreads), max_dynamic, s,
                                        static_cast<unsigned>(d.parts), op, d, scratch);
     }
     rc = launch_pdl(kv4_decode_kernel<kN, false>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s, op, d, scratch);
