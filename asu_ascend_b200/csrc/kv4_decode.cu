@@ -322,7 +322,6 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
         if (tc::elect_one()) {
             constexpr uint32_t kDescS = tc::instruction(128, kN, false, false);
             constexpr uint32_t kDescO = tc::instruction(128, kN, true, true);
-            constexpr uint32_t kHigh = tc::operand_high(128);
             const uint32_t desc_q = tc::operand(base + L::kQ, 0);
             const uint32_t desc_k = tc::operand(base + L::kRows, 0);
             const uint32_t desc_v = tc::operand(base + L::kRows, kBlock);
@@ -341,8 +340,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                         if (i == 4 && part == 0) continue;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            tc::mma_ss<kHigh, kHigh>(
-                                L::kColS, desc_k + (4 * part + i) * (kBlock / 16) + 2 * k,
+                            tc::mma_ss(L::kColS, desc_k + (4 * part + i) * (kBlock / 16) + 2 * k,
                                        desc_q + (4 * part + i) * (L::kQBlock / 16) + 2 * k, kDescS, part || i || k);
                     }
                 }
@@ -353,7 +351,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 for (int t = 0; t < 4; ++t) {
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc::mma_ss<kHigh, kHigh>(t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * (2048 / 16), kDescO,
+                        tc::mma_ss(t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * (2048 / 16), kDescO,
                                    !first || k);
                     if (t == 1) tc::commit(bar(kFreeLow));
                 }

@@ -228,7 +228,6 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
         if (tc::elect_one()) {
             constexpr uint32_t kDescS = tc::instruction(128, kTile, false, false);
             constexpr uint32_t kDescO = tc::instruction(128, 256, false, true);
-            constexpr uint32_t kHigh = tc::operand_high(128);
             const uint32_t desc_q = tc::operand(base + kSmemQ, 0);
             const uint32_t desc_a = tc::operand(base + kSmemA, 0);
             const uint32_t desc_b = tc::operand(base + kSmemB, 0);
@@ -240,14 +239,14 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tc::mma_ss<kHigh, kHigh>(kColS, desc_q + i * (kQBlock / 16) + 2 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+                        tc::mma_ss(kColS, desc_q + i * (kQBlock / 16) + 2 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
             };
             auto high = [&](uint32_t rows) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tc::mma_ts<kHigh>(kColS, kColQ + i * 32 + 8 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
+                        tc::mma_ts(kColS, kColQ + i * 32 + 8 * k, rows + i * (kBlock / 16) + 2 * k, kDescS, 1);
             };
             auto output = [&](uint32_t n, bool accumulate) {
                 wait(bar(kWeights), n);
@@ -255,7 +254,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 const uint32_t v = desc_v + (n & 1) * (4 * kBlock / 16);
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                    tc::mma_ts<kHigh>(kColO, kColP + 8 * k, v + k * (2048 / 16), kDescO, accumulate || k > 0);
+                    tc::mma_ts(kColO, kColP + 8 * k, v + k * (2048 / 16), kDescO, accumulate || k > 0);
                 tc::commit(bar2(kOutput, n));
             };
             uint32_t n = 0, segment = 0;
@@ -277,7 +276,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                     if (!part) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)  // rope; the tile's first product overwrites
-                            tc::mma_ts<kHigh>(kColS, kColQ + 4 * 32 + 8 * k, rows + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
+                            tc::mma_ts(kColS, kColQ + 4 * 32 + 8 * k, rows + 4 * (kBlock / 16) + 2 * k, kDescS, k > 0);
                     }
                     if ((half != 0) == (part == 0)) low(rows);
                     else high(rows);

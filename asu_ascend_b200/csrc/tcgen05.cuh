@@ -72,17 +72,7 @@ __device__ __forceinline__ void tmem_free(uint32_t base) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(kColumns) : "memory");
 }
 
-// 4, 8, 16 or 32 columns of the warp's 32 lanes: a thread holds one lane.
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr));
-}
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr));
-}
+// 16 or 32 columns of the warp's 32 lanes: a thread holds one lane.
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -123,12 +113,6 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[4]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
-}
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) : : "memory");
-}
 __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
 }
@@ -143,11 +127,8 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 __device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
     return ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);
 }
-// Rows of 128 bytes in the 128-byte swizzle (16-byte chunk ^ row % 8), or of 64 bytes in the 64-byte one
-// (chunk ^ row / 2 % 4); 8-row groups follow one another.
-__host__ __device__ constexpr uint32_t operand_high(int row_bytes) {
-    return (static_cast<uint32_t>(row_bytes) * 8 >> 4) | (1u << 14) | ((row_bytes == 128 ? 2u : 4u) << 29);
-}
+// Rows of 128 bytes in the 128-byte swizzle (16-byte chunk ^ row % 8); 8-row groups follow one another.
+constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 // kind::f16: bf16 x bf16 -> fp32, M x N, K = 16.
 __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_m_major, bool b_n_major) {
@@ -155,23 +136,21 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_m_major,
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-template <uint32_t kHighA, uint32_t kHighB>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{ .reg .pred p; .reg .b64 x, y; setp.ne.u32 p, %4, 0;\n"
         "mov.b64 x, {%1, %5}; mov.b64 y, {%2, %6};\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHighA), "n"(kHighB)
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh), "n"(kOperandHigh)
         : "memory");
 }
 // A in tensor memory: a lane a row of M, a column two values of K.
-template <uint32_t kHighB>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{ .reg .pred p; .reg .b64 y; setp.ne.u32 p, %4, 0;\n"
         "mov.b64 y, {%2, %5};\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHighB)
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kOperandHigh)
         : "memory");
 }
 // The barrier completes when every tcgen05.mma issued by this thread so far has.
