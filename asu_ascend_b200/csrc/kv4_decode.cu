@@ -696,9 +696,10 @@ Division division(int64_t tokens, int64_t topk, int sms) {
 
 void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
     const int64_t units = static_cast<int64_t>(d.rows) * d.tiles;
+    const int64_t pieces = d.parts == 1 ? 0 : 2ll * d.ctas;  // a CTA a token leaves none
     at[0] = 0;
-    at[1] = at[0] + align256(2ll * d.ctas * 2 * n * 4);
-    at[2] = at[1] + align256(2ll * d.ctas * n * kLatent * 4);
+    at[1] = at[0] + align256(pieces * 2 * n * 4);
+    at[2] = at[1] + align256(pieces * n * kLatent * 4);
     at[3] = at[2] + (weights ? align256(units * n * 4) : 0);
     at[4] = at[3] + (weights ? units * kTile * n * 2 : 0);
 }

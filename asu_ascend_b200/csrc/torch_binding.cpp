@@ -572,7 +572,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kv4_decode_cuda(const at::Tensor&
     if (T == 0) return {out, lse, w};
     // of this call alone, from the caching allocator: a captured graph's call gets its own from the graph's pool
     const int64_t size = asu_kv4_attention_workspace_bytes(T, H, K, weights);
-    at::Tensor ws = at::empty({size}, pool.options());
+    const at::Tensor ws = size > 0 ? at::empty({size}, pool.options()) : at::Tensor();
     const at::Tensor status = new_status(1, slots);
     launch_ok(asu_kv4_attention(c10::cuda::getCurrentCUDAStream(q.device().index()).stream(), q.data_ptr(),
                                 q.stride(0), q.stride(1), pool.data_ptr(), pool.size(-2), kv4_pitch(pool),
