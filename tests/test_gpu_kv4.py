@@ -92,6 +92,25 @@ def test_rows_match_the_oracle_byte_for_byte(kv4, checked, n, dtype, pad, offset
     assert np.array_equal(back.astype(np.float64), values)
 
 
+def test_every_magnitude_and_every_tie_is_rounded_as_the_definition_says(kv4, checked):
+    """Groups whose largest magnitude is each finite bf16 number in turn, and groups of all the ties of each scale:
+    the division by 7, the scale's rounding and the quotients, byte for byte."""
+    rng = np.random.default_rng(8)
+    top = torch.arange(1 << 15, dtype=torch.int32)[:0x7F80].to(torch.int16).view(torch.bfloat16)  # 0 to the largest
+    part = torch.from_numpy(rng.uniform(-1, 1, (top.numel(), 15)).astype(np.float32))
+    groups = torch.cat([top[:, None], (top.float()[:, None] * part).to(torch.bfloat16)], 1)
+    s = torch.from_numpy(O.scale_of(np.arange(256)).astype(np.float32))
+    ties = s[:, None] * (torch.arange(-7, 7) + 0.5)[None]  # 2k + 1 times a number of four bits: exact
+    ties = torch.cat([ties, 7 * s[:, None], -3 * s[:, None]], 1)
+    assert torch.equal(ties.to(torch.bfloat16).float(), ties)
+    groups = torch.cat([groups, ties.to(torch.bfloat16)])
+    x = torch.zeros(groups.shape[0] // 32, 576, dtype=torch.bfloat16)
+    x[:, :512] = groups.reshape(-1, 512)
+    pool = kv4.new_pool(x.shape[0], device=DEV)
+    kv4.pack_rows(x.to(DEV), pool)
+    assert np.array_equal(pool.cpu().numpy(), O.pack(x.float().numpy()))
+
+
 def test_every_code_and_scale_reads_back_exactly(kv4, checked):
     """256 rows, one per scale byte, with all nibbles."""
     b = np.zeros((256, 416), np.uint8)
