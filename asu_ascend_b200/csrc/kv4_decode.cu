@@ -166,9 +166,10 @@ __device__ __forceinline__ void join_in_cluster(const Operands& op, const Divisi
         for (int p = 0; p < parts; ++p) {
             float4 v[kHeads];
 #pragma unroll
-            for (int k = 0; k < kHeads; ++k)
-                v[k] = __ldcg(reinterpret_cast<const float4*>(
-                                  scratch.o + (static_cast<int64_t>(2 * (first_cta + p)) * kN + min(h0 + k, last - 1)) * kLatent) + t);
+            for (int k = 0; k < kHeads; ++k) {
+                const int64_t row = static_cast<int64_t>(2 * (first_cta + p)) * kN + min(h0 + k, last - 1);
+                v[k] = __ldcg(reinterpret_cast<const float4*>(scratch.o + row * kLatent) + t);
+            }
 #pragma unroll
             for (int k = 0; k < kHeads; ++k) {
                 const float f = s_factor[p][min(h0 + k, last - 1)];
@@ -189,7 +190,10 @@ __device__ __forceinline__ void join_in_cluster(const Operands& op, const Divisi
         uint4 v[kN / 8];
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) v[i] = __ldcg(p + i);
-        if (t < kN) s_tile[t] = s_lse[t] == -INFINITY ? 0.0f : exp2_fast(__ldcg(scratch.ref + static_cast<int64_t>(u) * kN + t) - s_lse[t]);
+        if (t < kN) {
+            const float ref = __ldcg(scratch.ref + static_cast<int64_t>(u) * kN + t);
+            s_tile[t] = s_lse[t] == -INFINITY ? 0.0f : exp2_fast(ref - s_lse[t]);
+        }
         asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
         const int e = (u - token * div.tiles) * kTile + t;
         float w = 0.0f;
@@ -351,8 +355,8 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 for (int t = 0; t < 4; ++t) {
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        tc::mma_ss(t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * (2048 / 16), kDescO,
-                                   !first || k);
+                        tc::mma_ss(t * kN, desc_v + t * (2 * kBlock / 16) + k * (2048 / 16), desc_p + k * (2048 / 16),
+                                   kDescO, !first || k);
                     if (t == 1) tc::commit(bar(kFreeLow));
                 }
                 tc::commit(bar(kOutput));
@@ -487,11 +491,13 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 const uint32_t to = base + L::kRope + tid * 128;
 #pragma unroll
                 for (int i = 0; i < kC / 8; ++i)
-                    shared_store16(to + (((c0 / 8 + i) ^ (tid & 7)) << 4), p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+                    shared_store16(to + (((c0 / 8 + i) ^ (tid & 7)) << 4), p[4 * i], p[4 * i + 1], p[4 * i + 2],
+                                   p[4 * i + 3]);
                 if (op.weights != nullptr) {
                     uint4* out = reinterpret_cast<uint4*>(scratch.p + (unit * kTile + tid) * kN + c0);
 #pragma unroll
-                    for (int i = 0; i < kC / 8; ++i) out[i] = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+                    for (int i = 0; i < kC / 8; ++i)
+                        out[i] = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
                 }
             }
             tc::fence_async_shared();
@@ -517,7 +523,8 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 if constexpr (kN == 16) s_top[warp][lane / 2] = __float_as_int(l[0]);
                 if constexpr (kN == 32) s_top[warp][lane] = __float_as_int(l[0]);
                 if constexpr (kN == 64)
-                    *reinterpret_cast<int2*>(&s_top[warp][2 * lane]) = make_int2(__float_as_int(l[0]), __float_as_int(l[1]));
+                    *reinterpret_cast<int2*>(&s_top[warp][2 * lane]) =
+                        make_int2(__float_as_int(l[0]), __float_as_int(l[1]));
                 softmax_sync();
                 const int row_start = token * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
@@ -629,10 +636,11 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
             load_ml(i, head);
             float4 v[kBatch];
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k)
-                v[k] = i + k <= i1 ? __ldcg(reinterpret_cast<const float4*>(
-                                                scratch.o + (static_cast<int64_t>(div.piece(i + k, first)) * kN + head) * kLatent) + tid)
+            for (int k = 0; k < kBatch; ++k) {
+                const int64_t row = static_cast<int64_t>(div.piece(i + k, first)) * kN + head;
+                v[k] = i + k <= i1 ? __ldcg(reinterpret_cast<const float4*>(scratch.o + row * kLatent) + tid)
                                    : make_float4(0, 0, 0, 0);
+            }
             join();
             acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
 #pragma unroll

@@ -437,8 +437,9 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
+                const float x = __uint_as_float(s[i / 16][2 * i % 32]), y = __uint_as_float(s[i / 16][(2 * i + 1) % 32]);
                 float a, b;
-                unpair(fma2(pair(__uint_as_float(s[i / 16][(2 * i) % 32]), __uint_as_float(s[i / 16][(2 * i + 1) % 32])), scale2, from2), a, b);
+                unpair(fma2(pair(x, y), scale2, from2), a, b);
                 a = exp2_fast(a);
                 b = exp2_fast(b);
                 l2 = add2(l2, pair(a, b));
@@ -571,9 +572,11 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
             float m0, l0, m1, l1, old, f0, f1, a[kCols], b[kCols];
             load_ml(i, m0, l0);
             load_ml(i + kStep, m1, l1);
-            const float* o0 = scratch.o + (static_cast<int64_t>(div.piece(i, first) * 2 + half) * 256 + c0) * 128 + head;
-            const float* o1 =
-                scratch.o + (static_cast<int64_t>(div.piece(i + kStep <= i1 ? i + kStep : i, first) * 2 + half) * 256 + c0) * 128 + head;
+            auto piece = [&](int k) {
+                return scratch.o + (static_cast<int64_t>(div.piece(k, first) * 2 + half) * 256 + c0) * 128 + head;
+            };
+            const float* o0 = piece(i);
+            const float* o1 = piece(i + kStep <= i1 ? i + kStep : i);
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
                 a[c] = __ldcg(o0 + c * 128);
@@ -660,7 +663,8 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
     if (group == 0) {
         const float lse = l > 0.0f && head < op.heads ? m + log2f(l) : -INFINITY;  // base 2
 #pragma unroll
-        for (int k = 0; k < kFinishTiles; ++k) s_shared[k * 128 + head] = lse == -INFINITY ? 0.0f : exp2_fast(ref[k] - lse);
+        for (int k = 0; k < kFinishTiles; ++k)
+            s_shared[k * 128 + head] = lse == -INFINITY ? 0.0f : exp2_fast(ref[k] - lse);
     }
     __syncthreads();
     for (int k0 = warp; k0 < count * 32; k0 += kBatch * kWarps) {
@@ -685,7 +689,8 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
 
 // Among pairs of CTAs, one for each half of the output columns.
 Division wide_division(int64_t tokens, int64_t topk, int sms) {
-    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms > 1 ? sms / 2 : 1, 3);  // no entry: an empty tile
+    const int64_t tiles = topk > 0 ? (topk + kTile - 1) / kTile : 1;  // no entry: an empty tile
+    return Division(tokens, tiles, sms > 1 ? sms / 2 : 1, 3);
 }
 
 // Byte offsets of the scratch arrays; [4] is the size.

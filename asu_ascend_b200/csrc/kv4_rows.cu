@@ -65,7 +65,8 @@ template <int kAlign>
 __device__ __forceinline__ void load16(const uint16_t* p, uint4 (&v)[2]) {
     if constexpr (kAlign == 32) {
         asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-            : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w)
+            : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z),
+              "=r"(v[1].w)
             : "l"(p));
     } else {
         v[0] = load8<kAlign>(p);
