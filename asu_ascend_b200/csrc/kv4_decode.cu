@@ -146,13 +146,13 @@ __device__ __forceinline__ void join_in_cluster(const Operands& op, const Divisi
             m[p] = m[p] == -INFINITY ? 0.0f : exp2_fast(m[p] - top);
             sum = fmaf(l[p], m[p], sum);
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a NaN goes on
 #pragma unroll
         for (int p = 0; p < kMaxParts; ++p) s_factor[p][h] = m[p] * inv;
-        s_lse[h] = sum > 0.0f && h < op.heads ? top + log2f(sum) : -INFINITY;
+        s_lse[h] = sum != 0.0f && h < op.heads ? top + log2f(sum) : -INFINITY;
         if (rank == 0 && h < op.heads)
             op.lse[static_cast<int64_t>(token) * op.heads + h] =
-                sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+                sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
     __syncthreads();
     const int t = threadIdx.x & 127, group = threadIdx.x >> 7;  // three groups, and a warp that looks on
@@ -206,7 +206,8 @@ __device__ __forceinline__ void join_in_cluster(const Operands& op, const Divisi
                 w = fmaf(__uint_as_float(x[k] & 0xffff0000u), s_tile[i * 8 + 2 * k + 1], w);
             }
         }
-        if (e < op.topk) op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(w);
+        if (e < op.topk)
+            op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(weight_of(op, token, e, w));
         asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
     }
 }
@@ -533,12 +534,12 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                     const float sum = (__int_as_float(s_top[0][tid]) + __int_as_float(s_top[1][tid])) +
                                       (__int_as_float(s_top[2][tid]) + __int_as_float(s_top[3][tid]));
                     if (whole) {
-                        s_fade[tid] = sum > 0.0f ? 1.0f / sum : 0.0f;
+                        s_fade[tid] = sum != 0.0f ? 1.0f / sum : 0.0f;  // a NaN goes on
                         if (tid < op.heads)
                             op.lse[static_cast<int64_t>(token) * op.heads + tid] =
-                                sum > 0.0f ? (log2f(sum) - s_minus_ref[tid]) * 0.6931471805599453f : -INFINITY;
+                                sum != 0.0f ? (log2f(sum) - s_minus_ref[tid]) * 0.6931471805599453f : -INFINITY;
                     } else {
-                        scratch.ml[piece * 2 * kN + tid] = sum > 0.0f ? -s_minus_ref[tid] : -INFINITY;
+                        scratch.ml[piece * 2 * kN + tid] = sum != 0.0f ? -s_minus_ref[tid] : -INFINITY;
                         scratch.ml[(piece * 2 + 1) * kN + tid] = sum;
                     }
                 }
@@ -649,12 +650,12 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
                 acc.z = fmaf(v[k].z, f[k], acc.z), acc.w = fmaf(v[k].w, f[k], acc.w);
             }
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
         reinterpret_cast<uint2*>(op.out + (static_cast<int64_t>(token) * op.heads + head) * kLatent)[tid] =
             make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
         if (tid == 0)
             op.lse[static_cast<int64_t>(token) * op.heads + head] =
-                l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
         return;
     }
     const int tile = 2 * (blockIdx.y - joins) + part;
@@ -675,7 +676,7 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
                     load_ml(i, tid);
                     join();
                 }
-                if (l > 0.0f) lse = m + log2f(l);
+                if (l != 0.0f) lse = m + log2f(l);
             }
         }
         s_factor[part][tid] = lse == -INFINITY ? 0.0f : exp2_fast(ref - lse);
@@ -693,7 +694,7 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
             w = fmaf(__uint_as_float(x[k] & 0xffff0000u), s_factor[part][i * 8 + 2 * k + 1], w);
         }
     }
-    op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(w);
+    op.weights[static_cast<int64_t>(token) * op.topk + e] = __float2bfloat16(weight_of(op, token, e, w));
 }
 
 int columns_of(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }

@@ -125,6 +125,14 @@ __device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Entry e's weight from the sum over the heads.  A head whose scores are not numbers makes the sum NaN, for entries that
+// are not there too (their 0 times its factor): those stay at 0.
+__device__ __forceinline__ float weight_of(const Operands& op, int64_t token, int e, float sum) {
+    if (sum == sum) return sum;
+    const int32_t s = __ldg(op.slots + token * op.slots_token + e);
+    return s >= 0 && s < op.pool_rows ? sum : 0.0f;
+}
+
 inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // kv4_decode.cu: up to kTallHeads heads

@@ -467,7 +467,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                 const int32_t row_start = at.row * tiles;
                 const bool whole = row_start >= u0 && row_start + tiles <= u1;
                 if (whole) {
-                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // a NaN goes on
                     __nv_bfloat16* out = op.out + (token * op.heads + head) * kLatent + half * 256;
 #pragma unroll 1
                     for (int c = 0; c < 256; c += 32) {
@@ -489,7 +489,7 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
                     }
                     if (half == 0 && head < op.heads)
                         op.lse[token * op.heads + head] =
-                            l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                            l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
                 } else {
                     const int piece = div.piece(blockIdx.x >> 1, row_start) * 2 + half;
                     float* to = scratch.o + static_cast<int64_t>(piece) * 256 * 128 + head;
@@ -612,7 +612,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
             }
         }
         if (head >= op.heads) return;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
         uint32_t w[kCols / 2];
 #pragma unroll
         for (int c = 0; c < kCols; c += 2) w[c / 2] = pack_bf16(acc[c] * inv, acc[c + 1] * inv);
@@ -620,7 +620,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
         if constexpr (kCols == 16) store32(out, w);
         else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
         if (y == 0 && c0 == 0)
-            op.lse[token * op.heads + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            op.lse[token * op.heads + head] = l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
         return;
     }
     const int tile0 = (y - kJoins) * kFinishTiles, count = min(kFinishTiles, div.tiles - tile0);
@@ -661,7 +661,7 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
         __syncthreads();
     }
     if (group == 0) {
-        const float lse = l > 0.0f && head < op.heads ? m + log2f(l) : -INFINITY;  // base 2
+        const float lse = l != 0.0f && head < op.heads ? m + log2f(l) : -INFINITY;  // base 2
 #pragma unroll
         for (int k = 0; k < kFinishTiles; ++k)
             s_shared[k * 128 + head] = lse == -INFINITY ? 0.0f : exp2_fast(ref[k] - lse);
@@ -682,7 +682,8 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             const int e = tile0 * kTile + 2 * k + (lane >> 4);
-            if ((lane & 15) == 0 && k < count * 32 && e < op.topk) op.weights[token * op.topk + e] = __float2bfloat16(sum);
+            if ((lane & 15) == 0 && k < count * 32 && e < op.topk)
+                op.weights[token * op.topk + e] = __float2bfloat16(weight_of(op, token, e, sum));
         }
     }
 }

@@ -414,3 +414,52 @@ def test_four_bit_rows_through_the_managed_cache(kv4, checked):
         ds = (576 * 2.0**-23 + 2.0**-22) * smag
         lim = (H_BF16 + 2 * ds[:, None] + 2 * 2.0**-16) * mag
         assert (np.abs(out[0].float().cpu().numpy() - o) <= lim + H_BF16 * (np.abs(o) + lim)).all()
+
+
+# ---- values that are not finite ----------------------------------------------------------------
+
+def plant(q, pool, slots, shift):
+    """NaN in a head's q, NaN in the rope part of a named row, an infinite value in a head's q, or nothing: by token."""
+    for t in range(q.shape[0]):
+        kind, h = (t + shift) % 4, (5 * t + shift) % q.shape[1]
+        live = slots[t][slots[t] >= 0]
+        if kind == 1:
+            q[t, h, 7] = float("nan")
+        elif kind == 2 and len(live):
+            pool[t, live[len(live) // 2], 290:292] = (0xC0, 0x7F)
+        elif kind == 3:
+            q[t, h, 512 + 5] = float("inf")
+            pool[t, :, 288 + 10: 288 + 12] = (0x80, 0x3F)  # times 1: an infinite score
+
+
+@pytest.mark.parametrize("T,H,K", [
+    (1, 16, 100), (1, 16, 700), (1, 64, 1500), (2, 33, 300), (37, 24, 777), (170, 16, 150), (150, 40, 260),
+    (1, 128, 60), (1, 128, 700), (3, 100, 300), (150, 80, 130)])
+def test_what_is_not_a_number_is_reported_as_such(kv4, checked, T, H, K):
+    """A head whose scores are not numbers has NaN for out and lse, and the weights of the token's entries are NaN;
+    entries that are not there keep weight 0, and other heads and tokens their values."""
+    for shift in (1, 2, 3) if T == 1 else (0, 2):
+        q, pool, slots = case(T, H, K, K + 50, True, 31 + T + H, 0.9)
+        plant(q, pool, slots, shift)
+        got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07,
+                                weights=True)
+        out, lse, w = (x.double().cpu().numpy() for x in got)
+        seen = 0
+        for t in range(T):
+            with np.errstate(invalid="ignore"):
+                o, l, ww, mag, smag = O.attention(q[t].float().numpy(), pool[t], slots[t], 0.07)
+            bad = np.isnan(l)
+            seen += bad.sum()
+            assert np.array_equal(np.isnan(lse[t]), bad), t
+            assert np.isnan(out[t][bad]).all(), t
+            ds = (576 * 2.0**-23 + 2.0**-22) * smag
+            lim = (H_BF16 + 2 * ds[:, None] + 2 * 2.0**-16) * mag
+            lim += H_BF16 * (np.abs(o) + lim)
+            assert (np.abs(out[t] - o) <= lim)[~bad].all(), t
+            assert (np.abs(lse[t] - l) <= ds + 2.0**-16 + 2.0**-22 * np.abs(l))[~bad].all(), t
+            assert not w[t][slots[t] < 0].any(), t
+            assert np.array_equal(np.isnan(w[t]), np.isnan(ww)), t
+            if not bad.any():
+                lim = ww * (2 * H_BF16 + 2 * ds.max() + 2.0**-16) * (1 + 2.0**-7) + H_BF16 * 2.0**-24 * H
+                assert (np.abs(w[t] - ww) <= lim).all(), t
+        assert seen > 0
