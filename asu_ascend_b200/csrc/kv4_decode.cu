@@ -50,6 +50,9 @@ constexpr int kThreads = 13 * 32;
 constexpr int kTile = 128;
 constexpr int kBlock = kTile * 128;  // bytes of a [128 entries x 64] block
 constexpr float kMaxGrowth = 40.0f;  // base 2
+// Minus the reference while there is none: any finite score exceeds it, and a score of -inf still gives a weight of 0
+// (with +inf here it would give NaN).
+constexpr float kNoReference = 3.4028235e38f;
 constexpr int kMaxParts = 8;         // CTAs of a cluster
 
 // Every barrier is waited for in every phase by each of its waiters, and its next phase depends on them: a
@@ -220,7 +223,7 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
-    __shared__ float s_minus_ref[kN];  // minus the reference, base 2; +inf while there is none
+    __shared__ float s_minus_ref[kN];  // minus the reference, base 2
     __shared__ float s_fade[kN];       // what a new reference multiplies sums and output by; later 1 / sum
     __shared__ __align__(8) int s_top[4][kN];       // each softmax warp's maximum, or sum
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -448,11 +451,10 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 softmax_sync();
                 if (tid < kN) {
                     const float top = unordered(max(max(s_top[0][tid], s_top[1][tid]), max(s_top[2][tid], s_top[3][tid])));
-                    // a piece whose entries so far are all missing has reference "none": minus it is +inf here,
-                    // so that the next score of any size exceeds it
-                    const float old = first ? INFINITY : s_minus_ref[tid];
+                    // a piece whose entries so far are all missing has none
+                    const float old = first ? kNoReference : s_minus_ref[tid];
                     const float now = fminf(old, -top);
-                    s_fade[tid] = old == now ? 1.0f : old == INFINITY ? 0.0f : exp2_fast(now - old);
+                    s_fade[tid] = old == now ? 1.0f : old == kNoReference ? 0.0f : exp2_fast(now - old);
                     s_minus_ref[tid] = now;
                 }
                 softmax_sync();

@@ -431,7 +431,8 @@ int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows, uint64_t p
  * with k_j all 576 values and v_j the first 512.  q: bf16, strides in elements; out [tokens, heads,
  * 512] bf16; lse [tokens, heads] fp32; weights [tokens, topk] bf16 (nullable).  A token without any
  * entry gets out 0, lse -inf and weights 0.  A head with a score that is NaN or +inf has NaN for out and lse, and the
- * weights of the token's entries are NaN (0 for those that are not there).  Any other slot outside [0, pool_rows) counts as not
+ * weights of the token's entries are NaN (0 for those that are not there); scores of -inf add nothing (scores are
+ * 32-bit sums).  Any other slot outside [0, pool_rows) counts as not
  * there and sets ASU_ST_BAD_QUERY in status[0] (nullable); ASU_ST_TIMEOUT there means that the kernel
  * gave up waiting for itself and that the outputs are not valid.  pool and its strides are 16-byte
  * aligned, out 32.  `workspace`: device memory of asu_kv4_attention_workspace_bytes(...) bytes on

@@ -463,3 +463,20 @@ def test_what_is_not_a_number_is_reported_as_such(kv4, checked, T, H, K):
                 lim = ww * (2 * H_BF16 + 2 * ds.max() + 2.0**-16) * (1 + 2.0**-7) + H_BF16 * 2.0**-24 * H
                 assert (np.abs(w[t] - ww) <= lim).all(), t
         assert seen > 0
+
+
+@pytest.mark.parametrize("T,H,K,split", [(1, 16, 300, 130), (3, 24, 777, 400), (170, 16, 300, 140), (2, 64, 260, 128),
+                                         (1, 128, 300, 70), (80, 100, 300, 140)])
+def test_scores_of_minus_infinity_add_nothing(kv4, checked, T, H, K, split):
+    """The first entries' scores overflow to -inf (2^127 times -4), for whole tiles and more: they count as if they were
+    not there, and a token that has no other entry gets what one without entries gets."""
+    q, pool, slots = case(T, H, K, K + 9, True, 71 + H)
+    q[:, :, 512] = 2.0**127
+    want = slots.copy()
+    for t in range(T):
+        n = K if t % 3 == 2 else split
+        pool[t, :, 288:290] = 0
+        pool[t, slots[t, :n], 288:290] = (0x80, 0xC0)  # -4
+        want[t, :n] = -1
+    got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07, weights=True)
+    check(q, pool, want, 0.07, got)
