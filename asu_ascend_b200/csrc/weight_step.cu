@@ -128,6 +128,7 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
     fill(s_hkey, s_hpos, kEmptyKey);
     fill(s_hpos, s_hval, INT32_MAX);  // and s_claim
     if (tid == 0) n_hits = n_valid = 0;
+    const int32_t tgt = static_cast<int32_t>(target < S ? target : S);
     if (free0 < 0 || free0 > static_cast<int32_t>(S)) {  // uniform across the block
         if (tid == 0) {
             flag_status(status, r, ASU_ST_BAD_STATE);
@@ -138,6 +139,7 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
             hit_mask[static_cast<uint64_t>(r) * Q + i] = 0;
             install_mask[static_cast<uint64_t>(r) * Q + i] = 0;
         }
+        for (int i = tid; i < tgt; i += kThreads) evicted[static_cast<uint64_t>(r) * ev_stride + i] = kNotFound;
         return;
     }
 #pragma unroll
@@ -232,7 +234,6 @@ weight_step_kernel(int32_t* __restrict__ t2s, int32_t* __restrict__ s2t, float* 
         __stcg(crow + slot_of(j), owner[j] < 0 ? 0.0f : v);
         if (owner[j] >= 0 && owner[j] < bound && !s_asked[slot_of(j)]) u[j] = __float_as_uint(v);
     }
-    const int32_t tgt = static_cast<int32_t>(target < S ? target : S);
     int32_t E = tgt > free0 ? tgt - free0 : 0;
     uint32_t cut = 0, whole = 0;  // the E-th lowest U among the candidates; all under `whole` leave
     int quota = 0;                // and so many of those at cut

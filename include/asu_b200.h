@@ -466,7 +466,8 @@ int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64
  * none): usually the slots of the step before and the weights that its attention gave them.
  * slot_out may be last_slot itself when last_count == query_count.  A weight that is negative,
  * infinite or NaN is not added and sets ASU_ST_BAD_WEIGHT; a last_slot outside [-1, slot_count)
- * sets ASU_ST_BAD_QUERY.  Results do not depend on scheduling.
+ * sets ASU_ST_BAD_QUERY.  A row whose free_count is out of range is left as it is and sets ASU_ST_BAD_STATE; its outputs
+ * say that no key has a slot and that none was evicted.  Results do not depend on scheduling.
  * Limits: slot_count <= 16384, query_count and last_count <= 4096, key_space < 2^31, decay in [0, 1]. */
 int asu_weight_step(void* stream, int32_t* token_to_slot, int32_t* slot_to_token, float* score, int32_t* free_stack,
                     int32_t* free_count, const int32_t* last_slot, const void* last_weight, int32_t weight_dtype,

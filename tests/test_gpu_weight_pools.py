@@ -271,3 +271,19 @@ def test_the_cache_the_attention_and_the_eviction_together(WeightSlotPools):
     pools.check_status()
     assert pools.totals()["evictions"] > 0
     host.close()
+
+
+def test_a_refused_row_lists_no_evicted_keys(WeightSlotPools):
+    """free_count out of range after a step that evicted: that row's outputs say that nothing left, the whole list."""
+    pools = WeightSlotPools(2, 100, 8, 3, 4, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    keys = torch.tensor([[0, 1, 2, 3], [5, 6, 7, 8]], **i32)
+    for step in range(3):
+        out = pools.step(keys + 10 * step)
+    assert out.evicted_count.tolist() == [3, 3] and (out.evicted >= 0).all()
+    pools.free_count[1] = -1
+    out = pools.step(keys + 30)
+    assert out.evicted_count.tolist() == [3, 0]
+    assert (out.evicted[0] >= 0).all() and (out.evicted[1] == -1).all()
+    with pytest.raises(RuntimeError, match="BAD_STATE"):
+        pools.check_status()
