@@ -6,6 +6,8 @@
 // A token without any entry: out 0, lse -inf, weights 0.
 #include "kv4_decode.cuh"
 
+#include <algorithm>
+
 using namespace asu;
 using namespace asu::kv4;
 
@@ -19,11 +21,29 @@ static int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, boo
     return heads <= kTallHeads ? tall_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
 }
 
+// Weights need the softmax weights of every head until a token's sum is known: two bytes a (padded) head and entry.
+// Calls of more tokens than kWeightsBytes of them hold are done in parts of the same size, one after the other
+// in the stream and in the same workspace.  128 heads x 2048 entries: 496 tokens, some 600 us of work a part.
+constexpr int64_t kWeightsBytes = 256ll << 20;
+static int64_t tokens_at_once(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+    if (!weights) return tokens;
+    const int64_t most = kWeightsBytes / (heads <= kTallHeads ? tall_weights(heads, topk) : wide_weights(topk));
+    const int64_t parts = (tokens + most - 1) / most;
+    return (tokens + parts - 1) / parts;
+}
+
+// Of the largest part, whether that is the last one or one before.
+static int64_t call_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
+    const int64_t some = tokens_at_once(tokens, heads, topk, weights), rest = tokens % some;
+    const int64_t bytes = decode_workspace(some, heads, topk, weights);
+    return rest > 0 ? std::max(bytes, decode_workspace(rest, heads, topk, weights)) : bytes;
+}
+
 extern "C" int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights) {
     if (tokens < 0 || heads < 0 || topk < 0 || tokens > ASU_KV4_MAX_TOKENS || heads > ASU_KV4_MAX_HEADS ||
         topk > ASU_KV4_MAX_TOPK)
         return -1;
-    return tokens && heads ? decode_workspace(tokens, heads, topk, weights != 0) : 0;
+    return tokens && heads ? call_workspace(tokens, heads, topk, weights != 0 && topk > 0) : 0;
 }
 
 extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -39,7 +59,8 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     if (!(scale_log2 > 0.0f) || !(scale_log2 < INFINITY)) return ASU_ERR_ARG;
     if (tokens == 0 || heads == 0) return ASU_OK;
     if (!q || !out || !lse || (topk && (!slots || !pool))) return ASU_ERR_ARG;
-    const int64_t need = decode_workspace(tokens, heads, topk, weights != nullptr);
+    if (topk == 0) weights = nullptr;
+    const int64_t need = call_workspace(tokens, heads, topk, weights != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_size < need)) return ASU_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(pool) % 16 || pool_pitch % 16 ||
         pool_token_stride % 16 || reinterpret_cast<uintptr_t>(out) % 32 || reinterpret_cast<uintptr_t>(lse) % 4 ||
@@ -57,14 +78,25 @@ extern "C" int asu_kv4_attention(void* stream, const void* q, int64_t q_token_st
     op.pool_rows = static_cast<int32_t>(pool_rows);
     op.slots = slots;
     op.slots_token = slots_token_stride;
-    op.tokens = static_cast<int32_t>(tokens);
     op.heads = static_cast<int32_t>(heads);
     op.topk = static_cast<int32_t>(topk);
     op.scale_log2 = scale_log2;
     op.q_aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     op.out = static_cast<__nv_bfloat16*>(out);
     op.lse = lse;
-    op.weights = topk ? static_cast<__nv_bfloat16*>(weights) : nullptr;
+    op.weights = static_cast<__nv_bfloat16*>(weights);
     op.status = status;
-    return op.heads <= kTallHeads ? launch_tall(s, op, workspace) : launch_wide(s, op, workspace);
+    const int64_t some = tokens_at_once(tokens, heads, topk, weights != nullptr);
+    for (int64_t t = 0; t < tokens; t += some) {
+        op.tokens = static_cast<int32_t>(std::min(some, tokens - t));
+        const int rc = op.heads <= kTallHeads ? launch_tall(s, op, workspace) : launch_wide(s, op, workspace);
+        if (rc != ASU_OK) return rc;
+        op.q += some * op.q_token;
+        op.pool += static_cast<uint64_t>(some) * op.pool_token;
+        op.slots += some * op.slots_token;
+        op.out += some * op.heads * kLatent;
+        op.lse += some * op.heads;
+        if (weights != nullptr) op.weights += some * op.topk;
+    }
+    return ASU_OK;
 }

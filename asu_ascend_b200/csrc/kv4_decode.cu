@@ -701,9 +701,9 @@ kv4_finish_kernel(const Operands op, const Division div, const Scratch scratch) 
 
 int columns_of(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
-Division division(int64_t tokens, int64_t topk, int sms) {
-    return Division(tokens, topk > 0 ? (topk + kTile - 1) / kTile : 1, sms, 1);  // no entry: one empty tile
-}
+int64_t tiles_of(int64_t topk) { return topk > 0 ? (topk + kTile - 1) / kTile : 1; }  // no entry: one empty tile
+
+Division division(int64_t tokens, int64_t topk, int sms) { return Division(tokens, tiles_of(topk), sms, 1); }
 
 void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
     const int64_t units = static_cast<int64_t>(d.rows) * d.tiles;
@@ -779,6 +779,8 @@ int64_t tall_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights
     layout(division(tokens, topk, asu_sm_count()), columns_of(heads), weights, at);
     return at[4];
 }
+
+int64_t tall_weights(int64_t heads, int64_t topk) { return tiles_of(topk) * columns_of(heads) * (4 + 2 * kTile); }
 
 int launch_tall(cudaStream_t s, const Operands& op, void* workspace) {
     switch (columns_of(op.heads)) {

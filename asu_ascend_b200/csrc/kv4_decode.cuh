@@ -138,9 +138,11 @@ inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 // kv4_decode.cu: up to kTallHeads heads
 constexpr int kTallHeads = 64;
 int64_t tall_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights);
+int64_t tall_weights(int64_t heads, int64_t topk);  // bytes of it for a token's weights
 int launch_tall(cudaStream_t stream, const Operands& op, void* workspace);
 // kv4_decode_wide.cu: more
 int64_t wide_workspace(int64_t tokens, int64_t topk, bool weights);
+int64_t wide_weights(int64_t topk);
 int launch_wide(cudaStream_t stream, const Operands& op, void* workspace);
 
 }  // namespace kv4

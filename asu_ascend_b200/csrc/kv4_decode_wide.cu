@@ -688,10 +688,11 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
     }
 }
 
+int64_t tiles_of(int64_t topk) { return topk > 0 ? (topk + kTile - 1) / kTile : 1; }  // no entry: an empty tile
+
 // Among pairs of CTAs, one for each half of the output columns.
 Division wide_division(int64_t tokens, int64_t topk, int sms) {
-    const int64_t tiles = topk > 0 ? (topk + kTile - 1) / kTile : 1;  // no entry: an empty tile
-    return Division(tokens, tiles, sms > 1 ? sms / 2 : 1, 3);
+    return Division(tokens, tiles_of(topk), sms > 1 ? sms / 2 : 1, 3);
 }
 
 // Byte offsets of the scratch arrays; [4] is the size.
@@ -710,6 +711,8 @@ int64_t wide_workspace(int64_t tokens, int64_t topk, bool weights) {
     wide_layout(wide_division(tokens, topk, asu_sm_count()), tokens, weights, at);
     return at[4];
 }
+
+int64_t wide_weights(int64_t topk) { return tiles_of(topk) * 128 * (4 + 2 * kTile); }
 
 int launch_wide(cudaStream_t s, const Operands& op, void* workspace) {
     const Division d = wide_division(op.tokens, op.topk, asu_sm_count());

@@ -65,6 +65,9 @@ def sparse_decode(q: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor, scal
     not there (a shorter context, a shortage).  An entry named twice counts twice.  With ``weights``
     the sum over the heads of each entry's softmax weight is returned too, 0 where there is no entry
     (heads sharded over ranks: add the ranks' weights).  A head with a score that is NaN or +inf has NaN
-    for ``out`` and ``lse``, and makes the weights of the token's entries NaN."""
+    for ``out`` and ``lse``, and makes the weights of the token's entries NaN.
+
+    With ``weights`` a call takes up to 256 MiB more of device memory while it runs: two bytes a head (of 16, 32, 64 or
+    128) and entry, and calls of more tokens than that holds are done in parts."""
     out, lse, w = torch.ops.asu.kv4_sparse_decode(q, pool, slots, scale, weights)
     return KV4Decode(out, lse, w if weights else None)

@@ -437,7 +437,7 @@ int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows, uint64_t p
  * gave up waiting for itself and that the outputs are not valid.  pool and its strides are 16-byte
  * aligned, out 32.  `workspace`: device memory of asu_kv4_attention_workspace_bytes(...) bytes on
  * the current device, 32-byte aligned, used by this call alone until it is done (-1: sizes out of
- * range).  Results do not depend on scheduling.
+ * range; 256 MiB at most for weights, and 39 MB on a B200 for tokens that several CTAs share).  Results do not depend on scheduling.
  * Limits: heads <= 128, tokens <= 65535, topk <= 16384. */
 int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights);
 int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* pool,

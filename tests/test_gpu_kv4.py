@@ -480,3 +480,46 @@ def test_scores_of_minus_infinity_add_nothing(kv4, checked, T, H, K, split):
         want[t, :n] = -1
     got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07, weights=True)
     check(q, pool, want, 0.07, got)
+
+
+# ---- many tokens in a call ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,H,K,own,part", [(4100, 16, 2048, False, 2050), (1100, 64, 2048, False, 550),
+                                            (700, 128, 2048, True, 350), (500, 128, 2048, False, 250)])
+def test_weights_of_more_tokens_than_the_workspace_holds(kv4, checked, T, H, K, own, part):
+    """Calls that are done in parts (256 MiB of softmax weights each): bit for bit the calls of those parts."""
+    S = 300
+    rng = np.random.default_rng(T)
+    pool = random_pool((T, S) if own else (S,), 3)
+    slots = rng.integers(-1, S, (T, K)).astype(np.int32)
+    q = torch.randn(H, T, 576, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).transpose(0, 1)
+    dq, dp = q.to(DEV), torch.from_numpy(pool).to(DEV)
+    ds = torch.full((T, K + 5), -9, dtype=torch.int32, device=DEV)[:, 2: K + 2]
+    ds.copy_(torch.from_numpy(slots))
+    got = kv4.sparse_decode(dq, dp, ds, 0.07, weights=True)
+    for t in range(0, T, part):
+        at = slice(t, t + part)
+        want = kv4.sparse_decode(dq[at], dp[at] if own else dp, ds[at], 0.07, weights=True)
+        for a, b in zip(got, want):
+            assert torch.equal(a[at], b)
+    at = [0, 1, part - 1, part, part + 1, T - 1]
+    some = kv4_of(got, at)
+    check(q[at], pool[at] if own else pool, slots[at], 0.07, some)
+
+
+def kv4_of(got, at):
+    return type(got)(*(x[at] for x in got))
+
+
+@pytest.mark.parametrize("T,H,K", [(65535, 1, 3), (5000, 20, 33), (3000, 70, 90)])
+def test_many_tokens(kv4, checked, T, H, K):
+    """A prompt's worth of tokens and the most that a call takes; a sample of them against the oracle."""
+    S = 200
+    rng = np.random.default_rng(T)
+    pool = random_pool((S,), 4)
+    slots = rng.integers(-1, S, (T, K)).astype(np.int32)
+    q = torch.randn(T, H, 576, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+    got = kv4.sparse_decode(q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07, weights=True)
+    assert not torch.isnan(got.out).any() and not torch.isnan(got.lse).any()
+    at = np.unique(np.concatenate([[0, 1, T - 2, T - 1], rng.integers(0, T, 60)])).tolist()
+    check(q[at], pool, slots[at], 0.07, kv4_of(got, at))

@@ -203,3 +203,14 @@ def test_weight_slot_pools_check_their_arguments():
             WeightSlotPools.from_state(z((R, 100), dtype=torch.int32), z((R, S), dtype=torch.int32), z((R, S)),
                                        z((R, S), dtype=torch.int32), z((R,), dtype=torch.int32),
                                        free_target=kw["free_target"], query_count=kw["query_count"], decay=kw["decay"])
+
+
+def test_attention_workspace_is_bounded_whatever_the_call(lib):
+    """256 MiB for the weights of the tokens that are done at once; the rest depends on the number of SMs alone."""
+    size = lib.lib.asu_kv4_attention_workspace_bytes
+    for heads in (1, 16, 17, 33, 64, 65, 128):
+        for topk in (1, 130, 2048, 16384):
+            for tokens in (1, 2, 500, 4096, 65535):
+                bare, both = size(tokens, heads, topk, 0), size(tokens, heads, topk, 1)
+                assert 0 <= bare <= 64 << 20 and bare <= both <= (256 + 64) << 20, (tokens, heads, topk, both)
+    assert size(65535, 128, 0, 1) == size(65535, 128, 0, 0)
