@@ -707,7 +707,7 @@ Division division(int64_t tokens, int64_t topk, int sms) { return Division(token
 
 void layout(const Division& d, int n, bool weights, int64_t (&at)[5]) {
     const int64_t units = static_cast<int64_t>(d.rows) * d.tiles;
-    const int64_t pieces = d.parts == 1 ? 0 : 2ll * d.ctas;  // a CTA a token leaves none
+    const int64_t pieces = d.shares() ? 2ll * d.ctas : 0;
     at[0] = 0;
     at[1] = at[0] + align256(pieces * 2 * n * 4);
     at[2] = at[1] + align256(pieces * n * kLatent * 4);
@@ -763,9 +763,7 @@ int launch(cudaStream_t s, const Operands& op, void* workspace) {
                                        static_cast<unsigned>(d.parts), op, d, scratch);
     }
     rc = launch_pdl(kv4_decode_kernel<kN, false>, dim3(d.ctas), dim3(kThreads), Layout<kN>::kBytes, s, op, d, scratch);
-    bool shared_rows = false;  // does any row lie in several CTAs' ranges?
-    for (int i = 1; i < d.ctas && !shared_rows; ++i) shared_rows = d.start(i) % d.tiles != 0;
-    if (rc != ASU_OK || (!shared_rows && op.weights == nullptr)) return rc;
+    if (rc != ASU_OK || (!d.shares() && op.weights == nullptr)) return rc;
     return launch_pdl(kv4_finish_kernel<kN>,
                       dim3(static_cast<unsigned>(op.tokens),
                            static_cast<unsigned>((op.heads + 1) / 2 + (op.weights != nullptr ? (d.tiles + 1) / 2 : 0))),

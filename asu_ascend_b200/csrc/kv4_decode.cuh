@@ -62,6 +62,9 @@ struct Division {
         const int32_t first = more * (each + 1);
         return u < first ? u / (each + 1) : more + (u - first) / each;
     }
+    // Does any row lie in several CTAs' ranges, so that there are pieces?  (Ranges of unequal sizes cannot all start with
+    // a row: the units are a multiple of `tiles`.)
+    bool shares() const { return parts > 0 ? parts > 1 : tiles > 1 && (more > 0 || each % tiles != 0); }
     // Scratch slot of CTA i's piece of a row that starts at unit `row_start`: a CTA's range holds at
     // most two pieces of rows, one at its start and one at its end.
     __host__ __device__ __forceinline__ int32_t piece(int32_t i, int32_t row_start) const {

@@ -697,9 +697,10 @@ Division wide_division(int64_t tokens, int64_t topk, int sms) {
 
 // Byte offsets of the scratch arrays; [4] is the size.
 void wide_layout(const Division& d, int64_t tokens, bool weights, int64_t (&at)[5]) {
+    const int64_t pieces = d.shares() ? 4ll * d.ctas : 0;  // of halves
     at[0] = 0;
-    at[1] = at[0] + align256(4ll * d.ctas * 256 * 4);
-    at[2] = at[1] + align256(4ll * d.ctas * 256 * 128 * 4);
+    at[1] = at[0] + align256(pieces * 256 * 4);
+    at[2] = at[1] + align256(pieces * 256 * 128 * 4);
     at[3] = at[2] + (weights ? align256(tokens * d.tiles * 128 * 4) : 0);
     at[4] = at[3] + (weights ? tokens * d.tiles * 32 * 128 * 4 : 0);
 }

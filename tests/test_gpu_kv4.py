@@ -523,3 +523,18 @@ def test_many_tokens(kv4, checked, T, H, K):
     assert not torch.isnan(got.out).any() and not torch.isnan(got.lse).any()
     at = np.unique(np.concatenate([[0, 1, T - 2, T - 1], rng.integers(0, T, 60)])).tolist()
     check(q[at], pool, slots[at], 0.07, kv4_of(got, at))
+
+
+@pytest.mark.parametrize("T,H,K", [(60, 128, 300), (74, 80, 64), (148, 128, 130), (200, 100, 64), (148, 16, 300),
+                                   (296, 40, 200)])
+def test_tokens_of_a_cta_each_or_several(kv4, checked, T, H, K):
+    """No token lies in several CTAs' ranges, so that the call has no pieces and, without weights, no workspace."""
+    from asu_ascend_b200 import _lib
+
+    assert _lib.lib.asu_kv4_attention_workspace_bytes(T, H, K, 0) == 0
+    q, pool, slots = case(T, H, K, 400, False, 17 + T, 0.9)
+    args = (q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07)
+    got = kv4.sparse_decode(*args, weights=True)
+    check(q, pool, slots, 0.07, got)
+    bare = kv4.sparse_decode(*args)
+    assert torch.equal(bare.out, got.out) and torch.equal(bare.lse, got.lse)

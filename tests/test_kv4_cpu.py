@@ -214,3 +214,11 @@ def test_attention_workspace_is_bounded_whatever_the_call(lib):
                 bare, both = size(tokens, heads, topk, 0), size(tokens, heads, topk, 1)
                 assert 0 <= bare <= 64 << 20 and bare <= both <= (256 + 64) << 20, (tokens, heads, topk, both)
     assert size(65535, 128, 0, 1) == size(65535, 128, 0, 0)
+
+
+def test_tokens_that_no_ctas_share_need_no_workspace(lib):
+    """One tile a token leaves nothing to join, whatever the number of SMs."""
+    size = lib.lib.asu_kv4_attention_workspace_bytes
+    for heads, tile in ((16, 128), (64, 128), (65, 64), (128, 64)):
+        for tokens in (1, 7, 200, 5000):
+            assert size(tokens, heads, tile, 0) == 0, (tokens, heads)
