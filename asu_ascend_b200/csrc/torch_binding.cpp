@@ -691,7 +691,7 @@ extern "C" void asu_torch_set_status_checks(int enabled) { g_status_checks.store
 extern "C" int asu_torch_status_checks() { return g_status_checks.load() ? 1 : 0; }
 
 // asu_weight_step on a device and its current stream (or the given one): WeightSlotPools.step's call.  The stream and the
-// device cost Python 4 us of its 13, and 0.3 here.  An exception becomes a code.
+// device cost Python 4 us of its 13, and 0.3 here.  An exception becomes a CUDA error's code: its own if it carries one.
 extern "C" int asu_torch_weight_step(int device, int has_stream, void* stream, int32_t* token_to_slot,
                                      int32_t* slot_to_token, float* score, int32_t* free_stack, int32_t* free_count,
                                      const int32_t* last_slot, const void* last_weight, int32_t weight_dtype,
@@ -707,7 +707,9 @@ extern "C" int asu_torch_weight_step(int device, int has_stream, void* stream, i
                                last_weight, weight_dtype, last_count, decay, keep_from, query, slot_out, hit_mask,
                                install_mask, evicted, evicted_stride, evicted_count, stats, status, req_num, key_space,
                                slot_count, query_count, free_target);
+    } catch (const c10::AcceleratorError& e) {
+        return ASU_ERR_CUDA_BASE + e.get_error_code();
     } catch (...) {
-        return ASU_ERR_ARG;
+        return ASU_ERR_CUDA_BASE + static_cast<int>(cudaErrorUnknown);
     }
 }

@@ -222,3 +222,15 @@ def test_tokens_that_no_ctas_share_need_no_workspace(lib):
     for heads, tile in ((16, 128), (64, 128), (65, 64), (128, 64)):
         for tokens in (1, 7, 200, 5000):
             assert size(tokens, heads, tile, 0) == 0, (tokens, heads)
+
+
+@pytest.mark.parametrize("device", [-7, 99])
+def test_a_device_that_cannot_be_used_is_not_called_a_wrong_argument(lib, device):
+    """The step's way to the device reports CUDA's error (no device, or an invalid one).  (A key space of 0, so that
+    nothing can be launched.)"""
+    from asu_ascend_b200 import ops
+
+    rc = ops.weight_step(device, 0, None, *[16] * 5, None, None, 2, 0, 0.5, None, *[16] * 5, 4, 16, None, None, 1, 0, 8, 4, 4)
+    assert rc > lib.ASU_ERR_CUDA_BASE
+    with pytest.raises(lib.AsuError, match="device|driver|unknown|GPU"):
+        lib.check(rc, "step")
