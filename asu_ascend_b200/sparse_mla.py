@@ -122,12 +122,14 @@ def sparse_mla_decode(q: torch.Tensor, ctx: _manager.ASULayerKVCacheContext, top
     FlashMLA-sparse heads are padded to a multiple of ``head_padding`` (128 on Blackwell) as vLLM's
     bf16 path does (flashmla_sparse.py:961-990).
     """
+    four_bit = kv_cache.dtype == torch.uint8 and tuple(kv_cache.shape[-1:]) == (kv4.ROW_BYTES,)
+    if not four_bit:  # before the resolver moves any row
+        from vllm.third_party.flashmla.flash_mla_interface import flash_mla_sparse_fwd
+
     slots = resolve_topk(ctx, topk_indices, block_table, kv_cache)
     t, h, d = q.shape
-    if kv_cache.dtype == torch.uint8 and kv_cache.shape[2] == kv4.ROW_BYTES:
+    if four_bit:
         return kv4.sparse_decode(q, ctx.managed_kv_cache_0, slots.view(t, -1), softmax_scale).out
-    from vllm.third_party.flashmla.flash_mla_interface import flash_mla_sparse_fwd
-
     if h % head_padding:
         hp = (h + head_padding - 1) // head_padding * head_padding
         qp = q.new_zeros((t, hp, d))

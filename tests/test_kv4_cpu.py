@@ -234,3 +234,26 @@ def test_a_device_that_cannot_be_used_is_not_called_a_wrong_argument(lib, device
     assert rc > lib.ASU_ERR_CUDA_BASE
     with pytest.raises(lib.AsuError, match="device|driver|unknown|GPU"):
         lib.check(rc, "step")
+
+
+def test_a_decode_without_its_attention_library_leaves_the_managed_cache_alone(monkeypatch):
+    """Rows that need FlashMLA-sparse: where it is not installed the call fails before the resolver moves rows.  4-bit
+    rows do not need it."""
+    import sys
+
+    from asu_ascend_b200 import sparse_mla
+
+    calls = []
+    monkeypatch.setitem(sys.modules, "vllm", None)
+    monkeypatch.setattr(sparse_mla, "resolve_topk", lambda *a: calls.append(a) or torch.zeros(1, 4, dtype=torch.int32))
+    q, topk = torch.zeros(1, 16, 576, dtype=torch.bfloat16), torch.zeros(1, 4, dtype=torch.int32)
+
+    class Ctx:
+        managed_kv_cache_0 = torch.zeros(64, 416, dtype=torch.uint8)
+
+    with pytest.raises(ImportError):
+        sparse_mla.sparse_mla_decode(q, Ctx, topk, topk[0], torch.zeros(2, 64, 576, dtype=torch.bfloat16), 0.1)
+    assert not calls
+    with pytest.raises(RuntimeError, match="needs CUDA"):
+        sparse_mla.sparse_mla_decode(q, Ctx, topk, topk[0], torch.zeros(2, 64, 416, dtype=torch.uint8), 0.1)
+    assert len(calls) == 1
