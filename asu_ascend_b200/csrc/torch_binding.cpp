@@ -28,7 +28,6 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
-#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <optional>
@@ -464,14 +463,18 @@ void check_kv4_pool(const at::Tensor& pool, const c10::Device& dev, bool per_tok
                 "pool rows must be 416 contiguous bytes, got ", pool.size(-1), " with stride ", pool.stride(-1));
     TORCH_CHECK(pool.size(-2) > 0, "pool has no rows");
     TORCH_CHECK(pool.stride(-2) >= ASU_KV4_ROW_BYTES || pool.size(-2) == 1, "pool rows must not overlap");
-    TORCH_CHECK(pool.stride(-2) % 16 == 0 && reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0 &&
-                    (pool.dim() == 2 || pool.stride(0) % 16 == 0),
+    TORCH_CHECK((pool.size(-2) == 1 || pool.stride(-2) % 16 == 0) &&
+                    reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0 &&
+                    (pool.dim() == 2 || pool.size(0) == 1 || pool.stride(0) % 16 == 0),
                 "pool rows must start at multiples of 16 bytes");
 }
 
-// Bytes between pool rows; a pool of one row may carry any stride.
+// Bytes between pool rows, and between the pools of tokens; a dimension of one element may carry any stride.
 uint64_t kv4_pitch(const at::Tensor& pool) {
-    return static_cast<uint64_t>(std::max<int64_t>(pool.stride(-2), ASU_KV4_ROW_BYTES));
+    return static_cast<uint64_t>(pool.size(-2) == 1 ? ASU_KV4_ROW_BYTES : pool.stride(-2));
+}
+uint64_t kv4_token_stride(const at::Tensor& pool) {
+    return pool.dim() == 3 && pool.size(0) > 1 ? static_cast<uint64_t>(pool.stride(0)) : 0;
 }
 
 void check_kv4_slots(const at::Tensor& slots, const c10::Device& dev) {
@@ -576,7 +579,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kv4_decode_cuda(const at::Tensor&
     const at::Tensor status = new_status(1, slots);
     launch_ok(asu_kv4_attention(c10::cuda::getCurrentCUDAStream(q.device().index()).stream(), q.data_ptr(),
                                 q.stride(0), q.stride(1), pool.data_ptr(), pool.size(-2), kv4_pitch(pool),
-                                pool.dim() == 3 ? static_cast<uint64_t>(pool.stride(0)) : 0,
+                                kv4_token_stride(pool),
                                 slots.data_ptr<int32_t>(), slots.stride(0), T, H, K, static_cast<float>(scale),
                                 out.data_ptr(), lse.data_ptr<float>(), weights && K ? w.data_ptr() : nullptr,
                                 size ? ws.data_ptr() : nullptr, size, status_ptr(status)),

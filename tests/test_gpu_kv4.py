@@ -538,3 +538,20 @@ def test_tokens_of_a_cta_each_or_several(kv4, checked, T, H, K):
     check(q, pool, slots, 0.07, got)
     bare = kv4.sparse_decode(*args)
     assert torch.equal(bare.out, got.out) and torch.equal(bare.lse, got.lse)
+
+
+def test_pools_of_one_row_or_one_token_with_odd_strides(kv4, checked):
+    """The strides of dimensions of one element do not reach the kernels."""
+    one = torch.zeros(416, 1, dtype=torch.uint8, device=DEV).t()
+    x = latents(1, 2).to(torch.bfloat16)
+    kv4.pack_rows(x.to(DEV), one)
+    want = O.pack(x.float().numpy())
+    assert np.array_equal(one.cpu().numpy(), want)
+    assert np.array_equal(kv4.unpack_rows(one).double().cpu().numpy(), O.unpack(want))
+    odd = torch.zeros(1280, dtype=torch.uint8, device=DEV).as_strided((1, 1, 416), (425, 7, 1))
+    odd.copy_(one[None])
+    slots = np.array([[0, -1, 0]], np.int32)
+    for H in (16, 128):
+        q = torch.randn(1, H, 576, generator=torch.Generator().manual_seed(H)).to(torch.bfloat16)
+        got = kv4.sparse_decode(q.to(DEV), odd, torch.from_numpy(slots).to(DEV), 0.07, weights=True)
+        check(q, want, slots, 0.07, got)

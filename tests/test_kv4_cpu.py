@@ -257,3 +257,20 @@ def test_a_decode_without_its_attention_library_leaves_the_managed_cache_alone(m
     with pytest.raises(RuntimeError, match="needs CUDA"):
         sparse_mla.sparse_mla_decode(q, Ctx, topk, topk[0], torch.zeros(2, 64, 416, dtype=torch.uint8), 0.1)
     assert len(calls) == 1
+
+
+def test_pools_of_one_row_or_one_token_may_have_any_stride_there():
+    """A dimension of one element is never walked, so its stride does not count."""
+    from asu_ascend_b200 import kv4
+
+    bf, i32 = torch.bfloat16, torch.int32
+    one = torch.zeros(416, 1, dtype=torch.uint8).t()
+    assert one.shape == (1, 416) and one.stride() == (1, 1)
+    odd = torch.zeros(3 * 425, dtype=torch.uint8).as_strided((1, 1, 416), (425, 424, 1))
+    for call in (lambda: kv4.pack_rows(torch.zeros(1, 576, dtype=bf), one), lambda: kv4.unpack_rows(one),
+                 lambda: kv4.sparse_decode(torch.zeros(1, 3, 576, dtype=bf), odd, torch.zeros(1, 5, dtype=i32), 1.0)):
+        with pytest.raises(RuntimeError, match="needs CUDA"):
+            call()
+    for pool in (odd.expand(2, 1, 416), torch.zeros(2000, dtype=torch.uint8).as_strided((2, 1, 416), (424, 1, 1))):
+        with pytest.raises(RuntimeError, match="needs CUDA" if pool.stride(0) == 0 else "multiples of 16"):
+            kv4.sparse_decode(torch.zeros(2, 3, 576, dtype=bf), pool, torch.zeros(2, 5, dtype=i32), 1.0)
