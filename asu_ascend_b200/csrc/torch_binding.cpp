@@ -28,6 +28,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <optional>
