@@ -274,3 +274,62 @@ def test_pools_of_one_row_or_one_token_may_have_any_stride_there():
     for pool in (odd.expand(2, 1, 416), torch.zeros(2000, dtype=torch.uint8).as_strided((2, 1, 416), (424, 1, 1))):
         with pytest.raises(RuntimeError, match="needs CUDA" if pool.stride(0) == 0 else "multiples of 16"):
             kv4.sparse_decode(torch.zeros(2, 3, 576, dtype=bf), pool, torch.zeros(2, 5, dtype=i32), 1.0)
+
+
+# ---- one wrong operand at a time ---------------------------------------------------------------
+
+ALIGNED = dict(q=64, pool=64, slots=64, out=64, lse=64, ws=64, weights=64)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a call without fault would launch on addresses that are none")
+def test_the_aligned_calls_are_refused_for_want_of_a_device_alone(lib):
+    assert _attention(lib.lib, **ALIGNED) > lib.ASU_ERR_CUDA_BASE
+    assert lib.lib.asu_kv4_pack(None, 64, 0, 576, 4, None, 64, 8, 416, None) > lib.ASU_ERR_CUDA_BASE
+    assert lib.lib.asu_kv4_unpack(None, 64, 8, 416, None, 4, 64, 576, None) > lib.ASU_ERR_CUDA_BASE
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=65), dict(pool=72), dict(pool=65), dict(pitch=424), dict(pitch=417), dict(pt=8), dict(pt=416 * 8 + 4),
+    dict(slots=66), dict(out=48), dict(out=80), dict(lse=66), dict(ws=48), dict(weights=65)], ids=str)
+def test_attention_rejects_each_operand_out_of_line(lib, bad):
+    assert _attention(lib.lib, **(ALIGNED | bad)) == lib.ASU_ERR_ALIGN
+
+
+@pytest.mark.parametrize("bad", [
+    dict(tokens=-1), dict(tokens=65536), dict(heads=-1), dict(heads=129), dict(topk=-1), dict(topk=16385), dict(rows=-1),
+    dict(rows=2**31), dict(qt=-1), dict(qh=-1), dict(st=-1), dict(pitch=400), dict(q=None), dict(out=None), dict(lse=None),
+    dict(slots=None), dict(pool=None), dict(ws=None), dict(size=0), dict(scale=0.0), dict(scale=-1.0),
+    dict(scale=float("inf")), dict(scale=float("nan")), dict(scale=3e38)], ids=str)
+def test_attention_rejects_each_argument_out_of_range(lib, bad):
+    assert _attention(lib.lib, **(ALIGNED | bad)) == lib.ASU_ERR_ARG
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(R=0), "must be positive"), (dict(K=0), "must be positive"), (dict(S=0), "must be positive"),
+    (dict(Q=0), "must be positive"), (dict(target=-1), "free_target >= 0"), (dict(S=16385), "slot_count <= 16384"),
+    (dict(Q=4097), "query_count <= 4096"), (dict(decay=1.5), "decay"), (dict(decay=-0.1), "decay"),
+    (dict(decay=float("nan")), "decay"), (dict(), None)], ids=str)
+def test_weight_slot_pools_reject_each_argument(bad, text):
+    """ValueErrors of the sizes, which come before the device's RuntimeError (the last case: nothing else is wrong)."""
+    from asu_ascend_b200.weight_pools import WeightSlotPools
+
+    a = dict(R=1, K=100, S=16, Q=8, target=4, decay=1.0) | bad
+    i32 = dict(dtype=torch.int32)
+    state = (torch.zeros(a["R"], a["K"], **i32), torch.zeros(a["R"], a["S"], **i32), torch.zeros(a["R"], a["S"]),
+             torch.zeros(a["R"], a["S"], **i32), torch.zeros(a["R"], **i32))
+    with pytest.raises(RuntimeError if text is None else ValueError, match=text or "lives in HBM"):
+        WeightSlotPools.from_state(*state, free_target=a["target"], query_count=a["Q"], decay=a["decay"])
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_weight_slot_pools_reject_each_state_tensor(which):
+    from asu_ascend_b200.weight_pools import WeightSlotPools
+
+    names = ("token_to_slot", "slot_to_token", "score", "free_stack", "free_count")
+    shapes = ((2, 100), (2, 16), (2, 16), (2, 16), (2,))
+    state = [torch.zeros(s, dtype=torch.float32 if n == "score" else torch.int32) for n, s in zip(names, shapes)]
+    good = state[which]
+    for wrong in (good.to(torch.float64), torch.stack([good, good], -1)[..., 0], good.to("meta")):
+        state[which] = wrong
+        with pytest.raises(RuntimeError, match="on meta" if which == 0 and wrong.is_meta else f"{names[which]} must be"):
+            WeightSlotPools.from_state(*state, free_target=4, query_count=8)
