@@ -555,3 +555,32 @@ def test_pools_of_one_row_or_one_token_with_odd_strides(kv4, checked):
         q = torch.randn(1, H, 576, generator=torch.Generator().manual_seed(H)).to(torch.bfloat16)
         got = kv4.sparse_decode(q.to(DEV), odd, torch.from_numpy(slots).to(DEV), 0.07, weights=True)
         check(q, want, slots, 0.07, got)
+
+
+# ---- several calls at once ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("shapes", [
+    [(1, 16, 700), (2, 16, 600), (9, 16, 1000)],                 # clusters of 6, 5 and 8
+    [(1, 16, 100), (2, 33, 300), (1, 64, 1024), (20, 24, 700)],  # of 1 (for the weights), 3, 8, 6
+    [(61, 64, 300), (37, 24, 777), (170, 16, 150)],              # clusters of 2; without clusters
+    [(2, 16, 600), (1, 128, 900), (37, 24, 777), (20, 40, 700), (80, 100, 130)]], ids=str)
+def test_calls_of_several_kernels_on_several_streams(kv4, shapes):
+    """Blocks that join in clusters, blocks that do not and the kernel for many heads, at the same time on the same SMs:
+    bit for bit the results of one after the other."""
+    calls = []
+    for i, (T, H, K) in enumerate(shapes):
+        q, pool, slots = case(T, H, K, K + 20, False, 300 + i, 0.95)
+        args = (q.to(DEV), torch.from_numpy(pool).to(DEV), torch.from_numpy(slots).to(DEV), 0.07)
+        calls.append((args, kv4.sparse_decode(*args, weights=True), kv4.sparse_decode(*args)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for turn in range(40):
+        i = turn * 3 % len(calls) if len(calls) % 3 else turn % len(calls)
+        with torch.cuda.stream(streams[turn % 4]):
+            got.append((i, kv4.sparse_decode(*calls[i][0], weights=turn % 5 != 0)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        args, full, bare = calls[i]
+        for a, b in zip(g, full if g.weights is not None else bare):
+            assert (a is None and b is None) or torch.equal(a, b)
