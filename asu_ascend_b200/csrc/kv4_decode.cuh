@@ -128,12 +128,15 @@ __device__ __forceinline__ uint4 load_unaligned(const __nv_bfloat16* p) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ __forceinline__ bool is_there(const Operands& op, int64_t token, int e) {
+    const int32_t s = __ldg(op.slots + token * op.slots_token + e);
+    return s >= 0 && s < op.pool_rows;
+}
+
 // Entry e's weight from the sum over the heads.  A head whose scores are not numbers makes the sum NaN, for entries that
 // are not there too (their 0 times its factor): those stay at 0.
 __device__ __forceinline__ float weight_of(const Operands& op, int64_t token, int e, float sum) {
-    if (sum == sum) return sum;
-    const int32_t s = __ldg(op.slots + token * op.slots_token + e);
-    return s >= 0 && s < op.pool_rows ? sum : 0.0f;
+    return sum == sum || is_there(op, token, e) ? sum : 0.0f;
 }
 
 inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }

@@ -682,9 +682,19 @@ kv4_finish_wide_kernel(const Operands op, const Division div, const Scratch scra
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             const int e = tile0 * kTile + 2 * k + (lane >> 4);
-            if ((lane & 15) == 0 && k < count * 32 && e < op.topk)
-                op.weights[token * op.topk + e] = __float2bfloat16(weight_of(op, token, e, sum));
+            if ((lane & 15) == 0 && k < count * 32 && e < op.topk) op.weights[token * op.topk + e] = __float2bfloat16(sum);
         }
+    }
+    // The factor of a head whose scores are not numbers, NaN in each tile, has made all sums NaN: entries that are not
+    // there stay at 0.  (Out of the loop above, where asking each sum cost 2 us of 162 with 128 tokens.)
+    const float4 f = *reinterpret_cast<const float4*>(s_shared + lane * 4);
+    const float any = f.x + f.y + f.z + f.w;
+    if (!__any_sync(0xffffffffu, any != any)) return;
+    __syncwarp();
+    for (int k = warp; k < count * 32; k += kWarps) {  // the warp's own stores
+        const int e = tile0 * kTile + 2 * k + lane;
+        if (lane < 2 && e < op.topk && !is_there(op, token, e))
+            op.weights[token * op.topk + e] = __float2bfloat16(0.0f);
     }
 }
 
