@@ -73,7 +73,7 @@ extern "C" const char* asu_status_string(int code) {
     switch (code) {
         case ASU_OK: return "ok";
         case ASU_ERR_ARG: return "invalid argument (null pointer or size out of range)";
-        case ASU_ERR_ALIGN: return "pointer or row size not 16-byte aligned";
+        case ASU_ERR_ALIGN: return "pointer or row size not aligned (to 16 bytes, or to what the entry point states)";
         case ASU_ERR_NOALLOC_CAPACITY:
             return "topk_numel exceeds the fixed scratch of asu_kv_resolver_noalloc (ASU_RESOLVER_NOALLOC_MAX_TOPK)";
         default: break;

@@ -12,11 +12,13 @@ using namespace asu;
 using namespace asu::kv4;
 
 // Up to kTallHeads heads the kernel whose products have the heads as columns, above it the one whose products
-// have them as 128 rows.  One and the other in us, 2048 entries (in brackets the heads taken 64 at a time):
-//   heads             16        32        64          80         128
-//   128 tokens  51 / 109  59 / 110  90 / 112  (167) / 113  (181) / 117
-//   32 tokens   20 /  37  21 /  37  30 /  38   (54) /  38   (56) /  39
-// For one token they are within 2 us of each other.
+// have them as 128 rows.  One and the other in us, 2048 entries, each token's rows in a pool of its own, inputs in
+// rotation (none in L2):
+//   heads             16        32         64        80       128
+//   128 tokens  55 / 120  63 / 122  101 / 128   - / 131   - / 139
+//   32 tokens   23 /  37  25 /  38   33 /  38   - /  39   - /  41
+// The first, taking 64 heads at a time, needed 167 and 54 us for 80 heads.  For one token they are within 2 us of each
+// other.
 static int64_t decode_workspace(int64_t tokens, int64_t heads, int64_t topk, bool weights) {
     return heads <= kTallHeads ? tall_workspace(tokens, heads, topk, weights) : wide_workspace(tokens, topk, weights);
 }

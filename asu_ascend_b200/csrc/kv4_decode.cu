@@ -25,11 +25,12 @@
 // 13 warps: 4 softmax, 8 that load rows into registers and dequantise (the next tile's loads are issued as
 // soon as a tile is stored, and fly during its products), one that issues the products.
 //
-// Tokens cut into 2 to 8 equal parts are joined by the cluster of their CTAs, if all clusters run at once: 61 x 64 x
-// 1024 31.1 -> 29.4 us, 32 x 32 x 2048 22.1 -> 20.8, with weights of an uncut token 1 x 16 x 100 13.5 -> 12.3.  Others
-// are joined by a second kernel, 5 to 8 us after the first.
+// Tokens cut into 2 to 8 equal parts are joined by the cluster of their CTAs, if all clusters run at once, others by a
+// second kernel, 5 to 8 us after the first.  The second kernel and the cluster, in us: 61 x 64 x 1024 over one pool 32.1 /
+// 29.5, with weights 39.2 / 36.8; the weights of an uncut token, 1 x 16 x 100, 12.9 / 11.4; 32 x 32 x 2048 over one pool 22.1
+// / 21.8, but over a pool a token 23.4 / 25.2.
 //
-// 128 tokens x 16 heads x 2048 entries take 55 us, 61 x 64 x 1024 29 us.
+// 128 tokens x 16 heads x 2048 entries take 55 us, 61 x 64 x 1024 29 us (inputs in rotation, none in L2).
 // A tile is a chain of 3.3 us: the output products of its first half 0.35, two halves to dequantise 0.7 to 0.85
 // each (shared memory: 128 KB stored, and the products' rows read at the same time), the scores' second half 0.45,
 // the softmax 0.45, four hand-overs of 0.15; the loads of rows are hidden.  Tried and slower, 16 heads: tiles of 64
@@ -480,6 +481,9 @@ kv4_decode_kernel(const Operands op, const Division div, const Scratch scratch) 
                 uint32_t s[kC];
                 tc::tmem_load(lanes + L::kColS + c0, s);
                 tc::tmem_wait_load(s);
+                // The weights are rounded to bf16, as the tensor cores take them beside bf16 rows: half a step, 2^-8 of
+                // each at most, which the sums average out (0.0020 off the exact output in the mean instead of the
+                // 0.0017 that the output's own rounding leaves).  Their sum l takes them before the rounding.
                 uint32_t p[kC / 2];
 #pragma unroll
                 for (int h = 0; h < kC; h += 2) {

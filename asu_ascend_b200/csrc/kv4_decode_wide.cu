@@ -31,7 +31,8 @@ namespace {
 //
 // The two CTAs of a pair walk the same tiles, so that the rows' second reading finds them in L2.
 //
-// 128 tokens x 128 heads x 2048 entries take 120 us, with weights 144.  A tile takes 1.7 us, in which the
+// 128 tokens x 128 heads x 2048 entries take 139 us, with weights 162 (inputs in rotation, none in L2; 120 and 150 where
+// the same rows are read again).  There a tile takes 1.7 us, in which the
 // issuing lane waits for the products and for nothing else: they would take 1.0 alone, but the traffic of shared
 // memory is 1.3 (q read again for every tile 0.4, rows dequantised 0.3 and read 0.4, 4-bit rows in and out 0.2).
 // A change of tokens takes 4 us (the next q's 147 KB, the output through the lanes), the start 5, the joining of
@@ -434,6 +435,8 @@ kv4_decode_wide_kernel(const Operands op, const Division div, const Scratch scra
             }
             const uint64_t scale2 = pair(op.scale_log2, op.scale_log2);
             const uint64_t from2 = pair(-from, -from);
+            // rounded to bf16, as the tensor cores take them beside bf16 rows (2^-8 of each at most, averaged out by the
+            // sums); their sum takes them before the rounding
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {

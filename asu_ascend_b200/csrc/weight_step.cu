@@ -9,8 +9,8 @@
 //       first, in query order), later ones are hits; an empty stack leaves slot -1
 //
 // One CTA of 1024 threads per row.  A request's step is a serial chain of dependent loads and block barriers
-// over a few dozen KB: 15 us on the device for 1 x 10240 slots and 17 for 128 x 8192 (from a cold L2), of which
-// the loads are 5 to 8, the threshold 3, and every instruction of all threads costs 8 cycles.
+// over a few dozen KB: a call takes 14 to 15 us for 1 x 10240 slots and 20 for 128 x 8192 (from a cold L2), of which
+// the loads are 5 to 8, the threshold 3 to 4, and every instruction of all threads costs 8 cycles.
 //  * A warp owns a run of slots and takes 32 of them at a time: loads are of whole lines, shared memory has
 //    no bank conflicts, and ranks in slot order need the ballots and one exchange of a count per warp.
 //    (With a run of slots for each thread, strided, and a sum over the block for every bit of the
