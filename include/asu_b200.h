@@ -430,14 +430,15 @@ int asu_kv4_unpack(void* stream, const void* pool, int64_t pool_rows, uint64_t p
  *   lse_th = log sum_j exp s_hj,  weights_tj = sum_h p_hj
  * with k_j all 576 values and v_j the first 512.  q: bf16, strides in elements; out [tokens, heads,
  * 512] bf16; lse [tokens, heads] fp32; weights [tokens, topk] bf16 (nullable).  A token without any
- * entry gets out 0, lse -inf and weights 0.  A head with a score that is NaN or +inf has NaN for out and lse, and the
- * weights of the token's entries are NaN (0 for those that are not there); scores of -inf add nothing (scores are
- * 32-bit sums).  Any other slot outside [0, pool_rows) counts as not
+ * entry gets out 0, lse -inf and weights 0.  A head with a score that is NaN or +inf has NaN for out
+ * and lse, and the weights of the token's entries are NaN (0 for those that are not there); scores of
+ * -inf add nothing (scores are 32-bit sums).  Any other slot outside [0, pool_rows) counts as not
  * there and sets ASU_ST_BAD_QUERY in status[0] (nullable); ASU_ST_TIMEOUT there means that the kernel
  * gave up waiting for itself and that the outputs are not valid.  pool and its strides are 16-byte
  * aligned, out 32.  `workspace`: device memory of asu_kv4_attention_workspace_bytes(...) bytes on
  * the current device, 32-byte aligned, used by this call alone until it is done (-1: sizes out of
- * range; 256 MiB at most for weights, and 39 MB on a B200 for tokens that several CTAs share).  Results do not depend on scheduling.
+ * range; 256 MiB at most for weights, and 39 MB on a B200 for tokens that several CTAs share).  Results
+ * do not depend on scheduling.
  * Limits: heads <= 128, tokens <= 65535, topk <= 16384. */
 int64_t asu_kv4_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t topk, int32_t weights);
 int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* pool,
@@ -466,8 +467,9 @@ int asu_kv4_attention(void* stream, const void* q, int64_t q_token_stride, int64
  * none): usually the slots of the step before and the weights that its attention gave them.
  * slot_out may be last_slot itself when last_count == query_count.  A weight that is negative,
  * infinite or NaN is not added and sets ASU_ST_BAD_WEIGHT; a last_slot outside [-1, slot_count)
- * sets ASU_ST_BAD_QUERY.  A row whose free_count is out of range is left as it is and sets ASU_ST_BAD_STATE; its outputs
- * say that no key has a slot and that none was evicted.  Results do not depend on scheduling.
+ * sets ASU_ST_BAD_QUERY.  A row whose free_count is out of range is left as it is and sets
+ * ASU_ST_BAD_STATE; its outputs say that no key has a slot and that none was evicted.  Results do not
+ * depend on scheduling.
  * Limits: slot_count <= 16384, query_count and last_count <= 4096, key_space < 2^31, decay in [0, 1]. */
 int asu_weight_step(void* stream, int32_t* token_to_slot, int32_t* slot_to_token, float* score, int32_t* free_stack,
                     int32_t* free_count, const int32_t* last_slot, const void* last_weight, int32_t weight_dtype,
